@@ -104,9 +104,9 @@ __device__ __forceinline__ float quick_gelu(float v) {
   return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.702f * 1.4426950408889634f * v));
 }
 
-// Two values at a time (r06): the epilogues run these on 128 accumulator values per lane while the matrix pipe idles -- 27 % of a tile's time for the
-// erf form (FLAVA / CoCa MLP-up), 12 % for QuickGELU (CLIP).  On float2 the multiplies / adds / fmas compile to v_pk_mul / v_pk_add / v_pk_fma_f32
-// (one issue slot for two values; IEEE-exact like their scalar forms); only rcp / exp2 and the |v| operand stay per value.
+// Two values at a time: the epilogues run these on 128 accumulator values per lane while the matrix pipe idles -- 27 % of a tile's time for the
+// erf form (FLAVA / CoCa MLP-up), 12 % for QuickGELU (CLIP).  The build has no packed fp32 instructions (multimodal_amd/build.py), so a pair takes
+// two issue slots; with them the FLAVA step was 0.75 % shorter (24.90 against 25.09 ms), the CLIP forward the same (13.30 against 13.31 ms).
 typedef __attribute__((ext_vector_type(2))) float f32x2;
 __device__ __forceinline__ f32x2 quick_gelu2(f32x2 v) {  // bit-identical to quick_gelu() per element (same operations in the same order)
   const f32x2 z = v * (-1.702f * 1.4426950408889634f);
@@ -203,20 +203,24 @@ __device__ __forceinline__ void store_act_copy(const GemmArgs& p, uint4 v, int m
 template <int MI, int NI, int TM, int TN>
 __device__ __forceinline__ void add_bias(f32x16 (&acc)[NI][MI], const GemmArgs& p, int n0, int wn, int lane, const char* bias_lds = nullptr) {
   const int half = lane >> 5;
-  if (p.bias != nullptr) {
+  // the branch holds the loads only: with the additions inside it the accumulators met their unchanged selves at its end, through copies that spilled
 #pragma unroll
-    for (int ni = 0; ni < NI; ++ni)
+  for (int ni = 0; ni < NI; ++ni) {
+    f32x4 bv[4] = {};
+    if (p.bias != nullptr) {
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const int n = n0 + wn * TN + ni * 32 + 4 * half + 8 * g;
-        f32x4 bv = {0.f, 0.f, 0.f, 0.f};
-        if (bias_lds != nullptr) bv = *reinterpret_cast<const f32x4*>(bias_lds + (wn * TN + ni * 32 + 4 * half + 8 * g) * 4);  // block-uniform
-        else if (n + 3 < p.N) bv = load4(p.bias + n);
-#pragma unroll
-        for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) acc[ni][mi][4 * g + j] += bv[j];
+        if (bias_lds != nullptr) bv[g] = *reinterpret_cast<const f32x4*>(bias_lds + (wn * TN + ni * 32 + 4 * half + 8 * g) * 4);  // block-uniform
+        else if (n + 3 < p.N) bv[g] = load4(p.bias + n);
       }
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+#pragma unroll
+      for (int mi = 0; mi < MI; ++mi)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[ni][mi][4 * g + j] += bv[g][j];
   }
 }
 
@@ -388,7 +392,7 @@ __device__ __forceinline__ void gemm_epilogue_lds(f32x16 (&acc)[NI][MI], const G
 #pragma unroll
       for (int mi = 0; mi < MI; ++mi)
 #pragma unroll
-        for (int r = 0; r < 16; r += 2) {  // (pairs: v_pk_mul / v_pk_add issue, bit-identical to quick_gelu() per value)
+        for (int r = 0; r < 16; r += 2) {  // (bit-identical to quick_gelu() per value)
           const f32x2 qg = quick_gelu2(f32x2{acc[ni][mi][r], acc[ni][mi][r + 1]});
           acc[ni][mi][r] = qg[0]; acc[ni][mi][r + 1] = qg[1];
         }

@@ -8,6 +8,8 @@ import sys
 from pathlib import Path
 
 ROOT = Path(__file__).resolve().parents[1]
+sys.path.insert(0, str(ROOT))
+from multimodal_amd.build import NO_PACKED_FP32  # noqa: E402
 
 
 def regs_of(tok: str):
@@ -76,6 +78,6 @@ if __name__ == "__main__":
         src = Path(sys.argv[1])
     else:
         src = Path("/tmp/mmamd_gemm.s")
-        subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", f"-I{ROOT / 'include'}", "-S", "--cuda-device-only",
+        subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", *NO_PACKED_FP32, f"-I{ROOT / 'include'}", "-S", "--cuda-device-only",
                         str(ROOT / "multimodal_amd" / "csrc" / "gemm.hip"), "-o", str(src)], check=True, capture_output=True)
     sys.exit(1 if check(src, "-v" in sys.argv) else 0)

@@ -9,11 +9,14 @@ from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 ROOT = Path(__file__).resolve().parents[1]
+sys.path.insert(0, str(ROOT))
+from multimodal_amd.build import NO_PACKED_FP32  # noqa: E402
+
 CSRC = ROOT / "multimodal_amd" / "csrc"
 
 
 def check(src: Path):
-    cmd = ["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", "-Rpass-analysis=kernel-resource-usage", "-c", str(src),
+    cmd = ["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "-fPIC", "--offload-arch=gfx950", *NO_PACKED_FP32, "-Rpass-analysis=kernel-resource-usage", "-c", str(src),
            "-o", f"/tmp/_spill_{src.stem}.o"]
     res = subprocess.run(cmd, capture_output=True, text=True)
     out = []
