@@ -579,6 +579,72 @@ int mmamd_group_mean_normalize(const float* x, int G, int T, int d, float* out, 
 int mmamd_scale_normalize(const float* x, float* y, int rows, int d, float scale, mmamd_stream_t stream);
 int mmamd_target_rank(const float* scores, int64_t ld, const int64_t* target, int R, int C, int32_t* rank, mmamd_stream_t stream);
 
+/* --- decoding with a paged key-value cache -------------------------------------------------------------------------------------
+ * The incremental form of the reference's decoders (MultiHeadAttentionWithCache, modules/layers/multi_head_attention.py:98-180:
+ * past_key_value concatenated per call) for serving: keys and values live in pages, a page table names the pages of each row
+ * (sequence), and rows can share pages.
+ *
+ * key_pages / value_pages: [pages, kv_heads, page_size, dim] with any page, head and token strides (elements; multiples of 16 bytes), dim contiguous,
+ * 16-byte aligned; dim 64, 96 or 128.  page_table int32 [rows, slots], row stride table_row_stride: token t of row r lies at place t % page_size of page
+ * page_table[r][t / page_size].  A page number outside [0, pages) holds no tokens: nothing is read or stored there and its positions take no part.
+ * slots * page_size <= 2^30. */
+typedef struct {
+  void* key_pages;
+  void* value_pages;
+  const int32_t* page_table;
+  int64_t key_page_stride, key_head_stride, key_token_stride;
+  int64_t value_page_stride, value_head_stride, value_token_stride;
+  int64_t table_row_stride;
+  int32_t dtype, pages, page_size, slots, kv_heads, dim;
+} mmamd_paged_cache;
+
+/* Attention of one new token per row:  out[r, h] = sum_t softmax_t(scale q[r, h] . K[r, t, h / G]) V[r, t, h / G],  G = heads / kv_heads.
+ * q [rows, heads, dim], out the same, contiguous; dtype as the pages.  With k and v ([rows, kv_heads, dim]) the row's new token is first stored at
+ * position lengths[r] and t runs over 0 .. lengths[r]; without, over 0 .. lengths[r] - 1.  A row with nothing visible (length 0 without k, negative
+ * lengths, no mapped page) gives zeros; a new token that has no place (lengths[r] negative or at the table's end, or its page not mapped) is neither
+ * stored nor seen.  Two rows must not have their new tokens in one place.  Softmax statistics and sums in fp32.
+ * Workspace: mmamd_paged_attention_workspace bytes (0 where the rows fill the chip by themselves), 16-byte aligned, one per call in flight. */
+int64_t mmamd_paged_attention_workspace(const mmamd_paged_cache* cache, int rows, int heads);
+int mmamd_paged_attention(const mmamd_paged_cache* cache, const int32_t* lengths, const void* q, int64_t q_row, int64_t q_head, const void* k,
+                          int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, void* out, int rows, int heads, float scale,
+                          void* workspace, int64_t workspace_bytes, mmamd_stream_t stream);
+/* Stores prompts: token j < counts[r] (counts NULL: all `tokens`) of row r, k / v [rows, tokens, kv_heads, dim] with any strides, goes to position
+ * start[r] + j.  Tokens without a place are dropped; nothing else is written. */
+int mmamd_paged_append(const mmamd_paged_cache* cache, const void* k, int64_t k_row, int64_t k_token, int64_t k_head, const void* v, int64_t v_row,
+                       int64_t v_token, int64_t v_head, const int32_t* start, const int32_t* counts, int rows, int tokens, mmamd_stream_t stream);
+
+/* The pages of a cache.  pool: [pages, blocks, page_size, row_bytes], contiguous (blocks: layers, keys / values, heads); refcounts int32 [pages]: in how
+ * many table entries a page stands, free where not positive.
+ * paged_fork builds the tables of `rows` new rows from the old ones: new row r continues old row parents[r] (-1, or any number outside: an empty
+ * row).  It shares the parent's full pages.  The partial last page goes to the parent's first child if no other row holds it, all others get a fresh
+ * page with a copy of its tokens.  Then fresh pages follow up to reserve_rows[r] (NULL: `reserve`) more tokens.  Entries behind are -1, pages of the
+ * old rows that nobody continues lose their references.  new_lengths[r] = the parent's length.  Fresh pages are the lowest free ones, in the order of the
+ * new table's entries; *shortage = how many could not be had (those entries are -1, their tokens lost).  The old state is not changed.
+ * paged_compact moves the live pages with the highest numbers into the lowest free places, so that they are pages 0 .. *live - 1; entries whose page is
+ * not live become -1.  The places that were left keep their values.
+ * Outputs must not overlap inputs.  Workspaces 16-byte aligned, one per call in flight. */
+int64_t mmamd_paged_fork_workspace(int old_rows, int rows, int slots, int pages);
+int mmamd_paged_fork(void* pool, int pages, int blocks, int page_size, int64_t row_bytes, const int32_t* table, int64_t table_row, const int32_t* lengths,
+                     const int32_t* refcounts, int old_rows, int slots, const int32_t* parents, int rows, const int32_t* reserve_rows, int reserve,
+                     int32_t* new_table, int32_t* new_lengths, int32_t* new_refcounts, int32_t* shortage, void* workspace, int64_t workspace_bytes,
+                     mmamd_stream_t stream);
+int64_t mmamd_paged_compact_workspace(int pages);
+int mmamd_paged_compact(void* pool, int pages, int64_t page_bytes, const int32_t* table, int64_t table_row, int rows, int slots, const int32_t* refcounts,
+                        int32_t* new_table, int32_t* new_refcounts, int32_t* live, void* workspace, int64_t workspace_bytes, mmamd_stream_t stream);
+
+/* One step of a beam search over groups x beams rows of logits [groups * beams, vocab] (fp32 or bf16, row stride ld).  A beam that goes on offers
+ * scores[b] + log_softmax(logits[b])[v] for every v, a finished one its own score for v = eos; all others -inf.  The `beams` (<= 32) highest by
+ * total / max(length, 1)^length_penalty (length: the continuation's) win, ties go to the lowest b * vocab + v.  A beam with score -inf or NaN, or whose
+ * logits have no finite log-sum-exp (a NaN or +inf among them, or nothing but -inf), offers -inf throughout.
+ * lengths int32, finished uint8, sequences int64 [groups, beams, tokens] (NULL: not kept) are reordered: outputs [groups, beams] each, out_parents the row
+ * (group * beams + beam) that is continued -- paged_fork's `parents` --, out_sequences with the new token at the parent's length (dropped if there is no
+ * room; nothing is added to a finished beam).  Outputs must not overlap inputs. */
+int64_t mmamd_beam_search_workspace(int groups, int beams, int vocab);
+int mmamd_beam_search_step(const void* logits, int dtype, int64_t ld, const float* scores, const int32_t* lengths, const uint8_t* finished,
+                           const int64_t* sequences, int tokens, int64_t eos, double length_penalty, int groups, int beams, int vocab, float* out_scores,
+                           int32_t* out_lengths, uint8_t* out_finished, int64_t* out_tokens, int32_t* out_parents, int64_t* out_sequences,
+                           void* workspace, int64_t workspace_bytes, mmamd_stream_t stream);
+
 /* Elementwise dtype conversion helper (fp32 <-> bf16), n elements. Used for weight packing. */
 int mmamd_convert(const void* src, int src_dtype, void* dst, int dst_dtype, int64_t n,
                   mmamd_stream_t stream);

@@ -134,6 +134,15 @@ PROTOTYPES = {
         _i,
         [_vp, _vp, _i, _vp, _vp, _i, _vp, _i, _i, _i, _i, _vp, _f, _i, _vp, _vp, _vp, _vp, _vp],
     ),
+    "mmamd_paged_attention_workspace": (_i64, [_vp, _i, _i]),
+    "mmamd_paged_attention": (_i, [_vp, _vp, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i64, _i64, _vp, _i, _i, _f, _vp, _i64, _vp]),
+    "mmamd_paged_append": (_i, [_vp, _vp, _i64, _i64, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i, _i, _vp]),
+    "mmamd_paged_fork_workspace": (_i64, [_i, _i, _i, _i]),
+    "mmamd_paged_fork": (_i, [_vp, _i, _i, _i, _i64, _vp, _i64, _vp, _vp, _i, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "mmamd_paged_compact_workspace": (_i64, [_i]),
+    "mmamd_paged_compact": (_i, [_vp, _i, _i64, _vp, _i64, _i, _i, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "mmamd_beam_search_workspace": (_i64, [_i, _i, _i]),
+    "mmamd_beam_search_step": (_i, [_vp, _i, _i64, _vp, _vp, _vp, _vp, _i, _i64, C.c_double, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp]),
     "mmamd_convert": (_i, [_vp, _i, _vp, _i, _i64, _vp]),
     "mmamd_timer_create": (_vp, []),
     "mmamd_timer_destroy": (None, [_vp]),

@@ -1,0 +1,347 @@
+// paged_pages.hip — the pages of a key-value cache: forking rows (with reserving and freeing) and compacting the pool.
+//
+// A page is free while its count in refcounts is not positive.  Everything that picks pages picks the lowest ones in a fixed order, so that results do
+// not depend on the order in which workgroups run; the only atomics are integer additions and minima.
+#include "paged.h"
+
+namespace mmamd {
+
+struct ForkParams {
+  char* pool;
+  const int32_t *table, *lengths, *refs, *parents, *reserve_rows;
+  int32_t *new_table, *new_lengths, *new_refs, *shortage;
+  int32_t *first, *children, *base, *src, *fresh, *found;  // workspace: two per old row, two per new row, the fresh pages and how many there are
+  int64_t table_row;
+  int old_rows, rows, pages, slots, reserve, fresh_max;
+  int64_t page_bytes, block_bytes, row_bytes;
+  int blocks;
+  FastDiv page;
+};
+
+// what a new row takes over and needs
+struct RowPlan {
+  int parent, n, full, rest, kept, want;  // kept: pages that hold its tokens; want: pages up to its reserved ones
+};
+__device__ __forceinline__ RowPlan plan_row(const ForkParams& p, int r) {
+  RowPlan w;
+  const int cap = p.slots * (int)p.page.d;
+  const int parent = p.parents[r];
+  w.parent = (uint32_t)parent < (uint32_t)p.old_rows ? parent : -1;
+  w.n = w.parent < 0 ? 0 : clamp_int(p.lengths[w.parent], 0, cap);
+  int more = p.reserve_rows != nullptr ? p.reserve_rows[r] : p.reserve;
+  more = clamp_int(more, 0, cap - w.n);
+  w.full = (int)div_by(p.page, (uint32_t)w.n);
+  w.rest = w.n - w.full * (int)p.page.d;
+  w.kept = w.full + (w.rest > 0 ? 1 : 0);
+  w.want = (int)div_by(p.page, (uint32_t)w.n + (uint32_t)more + p.page.d - 1u);
+  return w;
+}
+
+__device__ __forceinline__ int wave_scan(int v, int lane) {  // inclusive
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const int u = __shfl_up(v, o);
+    if (lane >= o) v += u;
+  }
+  return v;
+}
+// exclusive scan over the 1024 threads of a workgroup; total in every thread
+__device__ __forceinline__ int block_scan(int v, int* lds, int& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int inc = wave_scan(v, lane);
+  __syncthreads();
+  if (lane == 63) lds[wave] = inc;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < 16; ++w) {
+    const int x = lds[w];
+    before += w < wave ? x : 0;
+    all += x;
+  }
+  total = all;
+  return before + inc - v;
+}
+
+// Workgroup 0 plans: the lowest child of every parent, the pages each new row needs (numbered over the rows in order), the lowest free pages.  The
+// others copy the counts, which paged_fork_apply_kernel then changes by what the tables gain and lose.
+__global__ __launch_bounds__(1024) void paged_fork_plan_kernel(const ForkParams p) {
+  const int tid = threadIdx.x;
+  if (blockIdx.x > 0) {
+    for (int i = (blockIdx.x - 1) * 1024 + tid; i < p.pages; i += (gridDim.x - 1) * 1024) p.new_refs[i] = p.refs[i];
+    return;
+  }
+  __shared__ int lds[16];
+  for (int i = tid; i < p.old_rows; i += 1024) { p.first[i] = 0x7fffffff; p.children[i] = 0; }
+  __threadfence_block();
+  __syncthreads();
+  for (int r = tid; r < p.rows; r += 1024) {
+    const int parent = p.parents[r];
+    if ((uint32_t)parent < (uint32_t)p.old_rows) { atomicMin(&p.first[parent], r); atomicAdd(&p.children[parent], 1); }
+  }
+  __threadfence_block();
+  __syncthreads();
+  int needed = 0;
+  for (int r0 = 0; r0 < p.rows; r0 += 1024) {
+    const int r = r0 + tid;
+    int need = 0, src = -1;
+    if (r < p.rows) {
+      const RowPlan w = plan_row(p, r);
+      need = w.want > w.kept ? w.want - w.kept : 0;
+      if (w.rest > 0) {
+        const int id = p.table[w.parent * p.table_row + w.full];
+        if ((uint32_t)id < (uint32_t)p.pages && !(__hip_atomic_load(&p.first[w.parent], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == r && p.refs[id] == 1)) {
+          src = id;
+          ++need;
+        }
+      }
+      p.new_lengths[r] = w.n;
+    }
+    int total;
+    const int before = block_scan(need, lds, total);
+    if (r < p.rows) { p.base[r] = needed + before; p.src[r] = src; }
+    needed += total;
+  }
+  int found = 0;
+  for (int i0 = 0; i0 < p.pages && found < needed; i0 += 4096) {  // (both sides are the same in every thread)
+    int c[4], mine = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + tid * 4 + k;
+      c[k] = i < p.pages && p.refs[i] <= 0;
+      mine += c[k];
+    }
+    int total;
+    int at = found + block_scan(mine, lds, total);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (c[k]) {
+        if (at < p.fresh_max) p.fresh[at] = i0 + tid * 4 + k;
+        ++at;
+      }
+    found += total;
+  }
+  if (found > needed) found = needed;
+  if (tid == 0) { p.found[0] = found; p.shortage[0] = needed - found; }
+}
+
+// grid (x, rows): x = 0 writes the row's table and its counts, every x copies its share of the row's partial page.  Rows beyond p.rows stand for the old
+// rows, whose references go.
+__global__ __launch_bounds__(256) void paged_fork_apply_kernel(const ForkParams p) {
+  const int tid = threadIdx.x;
+  if ((int)blockIdx.y >= p.rows) {
+    if (blockIdx.x > 0) return;
+    const int o = blockIdx.y - p.rows;
+    const int heirs = p.children[o];
+    const int cap = p.slots * (int)p.page.d;
+    const int n = clamp_int(p.lengths[o], 0, cap), full = (int)div_by(p.page, (uint32_t)n), rest = n - full * (int)p.page.d;
+    for (int j = tid; j < p.slots; j += 256) {
+      const int id = p.table[o * p.table_row + j];
+      if ((uint32_t)id >= (uint32_t)p.pages) continue;
+      int gain = -1;
+      if (j < full) gain += heirs;
+      else if (j == full && rest > 0 && heirs > 0 && p.refs[id] == 1) gain += 1;
+      if (gain != 0) atomicAdd(&p.new_refs[id], gain);
+    }
+    return;
+  }
+  const int r = blockIdx.y;
+  const RowPlan w = plan_row(p, r);
+  const int src = p.src[r], base = p.base[r], found = p.found[0];
+  if (blockIdx.x == 0) {
+    for (int j = tid; j < p.slots; j += 256) {
+      int id = -1;
+      if (j < w.kept && !(j == w.full && src >= 0)) {
+        id = p.table[w.parent * p.table_row + j];
+        if ((uint32_t)id >= (uint32_t)p.pages) id = -1;
+      } else if (j < w.want || (j == w.full && src >= 0)) {
+        const int at = base + (src >= 0 ? j - w.full : j - w.kept);
+        if (at < found) {
+          id = p.fresh[at];
+          atomicAdd(&p.new_refs[id], 1);
+        }
+      }
+      p.new_table[(int64_t)r * p.slots + j] = id;
+    }
+  }
+  if (src < 0 || base >= found) return;
+  const int dst = p.fresh[base];
+  const char* from = p.pool + src * p.page_bytes;
+  char* to = p.pool + dst * p.page_bytes;
+  const int per = (int)(w.rest * p.row_bytes / 16);  // 16-byte pieces of a block's tokens
+  for (int b = blockIdx.x; b < p.blocks; b += gridDim.x)
+    for (int i = tid; i < per; i += 256)
+      *reinterpret_cast<uint4*>(to + b * p.block_bytes + i * 16) = *reinterpret_cast<const uint4*>(from + b * p.block_bytes + i * 16);
+}
+
+struct CompactParams {
+  char* pool;
+  const int32_t *table, *refs;
+  int32_t *new_table, *new_refs, *live;
+  int32_t *counts, *rank, *src, *dst;  // workspace: live pages per block, per page, moved pages
+  int64_t table_row, page_bytes;
+  int rows, slots, pages, nblk;
+};
+constexpr int kCompactPer = 1024;  // pages per workgroup of the first two kernels
+
+__global__ __launch_bounds__(1024) void paged_compact_count_kernel(const CompactParams p) {
+  __shared__ int lds[16];
+  const int i = blockIdx.x * kCompactPer + threadIdx.x;
+  int total;
+  block_scan(i < p.pages && p.refs[i] > 0, lds, total);
+  if (threadIdx.x == 0) p.counts[blockIdx.x] = total;
+}
+
+// With M live pages: the k-th live page from M on moves to the k-th free place before M.  Lists both, and numbers the movers.
+__global__ __launch_bounds__(1024) void paged_compact_plan_kernel(const CompactParams p) {
+  __shared__ int lds[16];
+  __shared__ int sums[2];
+  const int tid = threadIdx.x, blk = blockIdx.x;
+  int all = 0, before = 0;
+  for (int b0 = 0; b0 < p.nblk; b0 += 1024) {
+    const int b = b0 + tid;
+    const int c = b < p.nblk ? p.counts[b] : 0;
+    int total;
+    const int ex = block_scan(c, lds, total);
+    if (b == blk) sums[0] = before + ex;
+    all += total;
+    before += total;
+  }
+  __syncthreads();
+  const int mine = sums[0];                     // live pages before this workgroup's
+  const int M = all;
+  const int i = blk * kCompactPer + tid;
+  const bool live = i < p.pages && p.refs[i] > 0;
+  int total;
+  const int l = mine + block_scan(live, lds, total);   // live pages before page i
+  // live pages before M: from the back, M minus the ones from M on; counted by the workgroup that holds page M, and by nobody where M = pages
+  const int mb = M / kCompactPer;
+  int lowest = 0;
+  for (int b0 = 0; b0 < mb; b0 += 1024) {
+    const int b = b0 + tid;
+    int t;
+    block_scan(b < mb ? p.counts[b] : 0, lds, t);
+    lowest += t;
+  }
+  {
+    const int x = mb * kCompactPer + tid;
+    int t;
+    block_scan(x < M && x < p.pages && p.refs[x] > 0, lds, t);
+    lowest += t;
+  }
+  if (i < p.pages) {
+    int rank = 0;  // of a mover among the movers, of a hole among the holes
+    if (live && i >= M) { rank = l - lowest; p.src[rank] = i; }
+    else if (!live && i < M) { rank = i - l; p.dst[rank] = i; }
+    p.rank[i] = rank;
+  }
+  if (blk == 0 && tid == 0) { p.live[0] = M; p.counts[p.nblk] = M - lowest; }
+}
+
+__global__ __launch_bounds__(256) void paged_compact_apply_kernel(const CompactParams p, int64_t pieces) {
+  const int M = p.live[0], moves = p.counts[p.nblk];
+  const int64_t step = (int64_t)gridDim.x * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  for (int64_t i = first; i < (int64_t)p.rows * p.slots; i += step) {
+    const int r = (int)(i / p.slots), j = (int)(i - (int64_t)r * p.slots);
+    int id = p.table[r * p.table_row + j];
+    if ((uint32_t)id >= (uint32_t)p.pages || p.refs[id] <= 0) id = -1;
+    else if (id >= M) id = p.dst[p.rank[id]];
+    p.new_table[i] = id;
+  }
+  for (int64_t i = first; i < p.pages; i += step) p.new_refs[i] = i >= M ? 0 : p.refs[i] > 0 ? p.refs[i] : p.refs[p.src[p.rank[i]]];
+  for (int k = blockIdx.x; k < moves; k += gridDim.x) {
+    const char* from = p.pool + p.src[k] * p.page_bytes;
+    char* to = p.pool + p.dst[k] * p.page_bytes;
+    for (int64_t i = threadIdx.x; i < pieces; i += 256) *reinterpret_cast<uint4*>(to + i * 16) = *reinterpret_cast<const uint4*>(from + i * 16);
+  }
+}
+
+}  // namespace mmamd
+
+using namespace mmamd;
+
+static int64_t up4(int64_t n) { return (n + 3) & ~3ll; }
+
+// most fresh pages that one call can give
+static int64_t fork_fresh(int rows, int slots, int pages) {
+  const int64_t n = (int64_t)rows * slots;
+  return n < pages ? n : pages;
+}
+
+extern "C" int64_t mmamd_paged_fork_workspace(int old_rows, int rows, int slots, int pages) {
+  MMAMD_CHECK_ARG(old_rows >= 0 && rows >= 0 && slots >= 1 && pages >= 1, MMAMD_E_BADARG, "mmamd_paged_fork_workspace: rows %d -> %d, slots %d, pages %d", old_rows, rows, slots, pages);
+  return 4 * (2 * up4(old_rows) + 2 * up4(rows) + up4(fork_fresh(rows, slots, pages)) + 4);
+}
+
+extern "C" int mmamd_paged_fork(void* pool, int pages, int blocks, int page_size, int64_t row_bytes, const int32_t* table, int64_t table_row, const int32_t* lengths,
+                                const int32_t* refcounts, int old_rows, int slots, const int32_t* parents, int rows, const int32_t* reserve_rows, int reserve,
+                                int32_t* new_table, int32_t* new_lengths, int32_t* new_refcounts, int32_t* shortage, void* workspace, int64_t workspace_bytes,
+                                mmamd_stream_t stream) {
+  MMAMD_CHECK_ARG(pages >= 1 && blocks >= 1 && page_size >= 1 && slots >= 1 && old_rows >= 0 && rows >= 0, MMAMD_E_BADARG,
+                  "mmamd_paged_fork: pages %d, blocks %d, page size %d, slots %d, rows %d -> %d", pages, blocks, page_size, slots, old_rows, rows);
+  MMAMD_CHECK_ARG((int64_t)slots * page_size <= 1 << 30 && (int64_t)rows + old_rows <= 65535 && (int64_t)rows * slots <= 0x7fffffffll && pages <= 0x7fffffff - 65536 && (int64_t)page_size * row_bytes <= 0x7fffffffll, MMAMD_E_UNSUPPORTED,
+                  "mmamd_paged_fork: %d slots of %d tokens, %d rows -> %d", slots, page_size, old_rows, rows);
+  MMAMD_CHECK_ARG(pool != nullptr && refcounts != nullptr && new_refcounts != nullptr && shortage != nullptr && workspace != nullptr, MMAMD_E_BADARG, "mmamd_paged_fork: null argument");
+  MMAMD_CHECK_ARG((old_rows == 0 || (table != nullptr && lengths != nullptr)) && (rows == 0 || (parents != nullptr && new_table != nullptr && new_lengths != nullptr)), MMAMD_E_BADARG,
+                  "mmamd_paged_fork: null argument");
+  MMAMD_CHECK_ARG(aligned16(pool) && row_bytes > 0 && row_bytes % 16 == 0, MMAMD_E_ALIGN, "mmamd_paged_fork: the pool must be 16-byte aligned, a token %lld bytes (multiples of 16)", (long long)row_bytes);
+  MMAMD_CHECK_ARG(workspace_bytes >= mmamd_paged_fork_workspace(old_rows, rows, slots, pages) && aligned16(workspace), MMAMD_E_BADARG, "mmamd_paged_fork: workspace of %lld bytes is too small",
+                  (long long)workspace_bytes);
+  ForkParams p;
+  p.pool = reinterpret_cast<char*>(pool);
+  p.table = table; p.lengths = lengths; p.refs = refcounts; p.parents = parents; p.reserve_rows = reserve_rows;
+  p.new_table = new_table; p.new_lengths = new_lengths; p.new_refs = new_refcounts; p.shortage = shortage;
+  int32_t* w = reinterpret_cast<int32_t*>(workspace);
+  p.first = w; w += up4(old_rows);
+  p.children = w; w += up4(old_rows);
+  p.base = w; w += up4(rows);
+  p.src = w; w += up4(rows);
+  p.found = w; w += 4;
+  p.fresh = w;
+  p.fresh_max = (int)fork_fresh(rows, slots, pages);
+  p.table_row = table_row;
+  p.old_rows = old_rows; p.rows = rows; p.pages = pages; p.slots = slots; p.reserve = reserve;
+  p.row_bytes = row_bytes; p.block_bytes = row_bytes * page_size; p.page_bytes = p.block_bytes * blocks; p.blocks = blocks;
+  p.page = fast_div((uint32_t)page_size);
+  hipStream_t st = (hipStream_t)stream;
+  int copiers = (pages + 4095) / 4096;
+  if (copiers > 64) copiers = 64;
+  paged_fork_plan_kernel<<<1 + copiers, 1024, 0, st>>>(p);
+  if (int rc = launch_status("paged_fork plan")) return rc;
+  if (rows + old_rows == 0) return 0;
+  const int gx = blocks < 64 ? blocks : 64;
+  paged_fork_apply_kernel<<<dim3(gx, rows + old_rows), 256, 0, st>>>(p);
+  return launch_status("paged_fork");
+}
+
+extern "C" int64_t mmamd_paged_compact_workspace(int pages) {
+  MMAMD_CHECK_ARG(pages >= 1, MMAMD_E_BADARG, "mmamd_paged_compact_workspace: pages %d", pages);
+  return 4 * (up4((pages + kCompactPer - 1) / kCompactPer + 1) + 3 * up4(pages));
+}
+
+extern "C" int mmamd_paged_compact(void* pool, int pages, int64_t page_bytes, const int32_t* table, int64_t table_row, int rows, int slots, const int32_t* refcounts,
+                                   int32_t* new_table, int32_t* new_refcounts, int32_t* live, void* workspace, int64_t workspace_bytes, mmamd_stream_t stream) {
+  MMAMD_CHECK_ARG(pages >= 1 && rows >= 0 && slots >= 1 && page_bytes > 0, MMAMD_E_BADARG, "mmamd_paged_compact: pages %d of %lld bytes, %d rows of %d slots", pages, (long long)page_bytes, rows, slots);
+  MMAMD_CHECK_ARG(pages <= 0x7fffffff - 65536, MMAMD_E_UNSUPPORTED, "mmamd_paged_compact: %d pages", pages);
+  MMAMD_CHECK_ARG(pool != nullptr && refcounts != nullptr && new_refcounts != nullptr && live != nullptr && workspace != nullptr && (rows == 0 || (table != nullptr && new_table != nullptr)),
+                  MMAMD_E_BADARG, "mmamd_paged_compact: null argument");
+  MMAMD_CHECK_ARG(aligned16(pool) && page_bytes % 16 == 0, MMAMD_E_ALIGN, "mmamd_paged_compact: the pool must be 16-byte aligned, with pages of whole 16-byte pieces");
+  MMAMD_CHECK_ARG(workspace_bytes >= mmamd_paged_compact_workspace(pages) && aligned16(workspace), MMAMD_E_BADARG, "mmamd_paged_compact: workspace of %lld bytes is too small", (long long)workspace_bytes);
+  CompactParams p;
+  p.pool = reinterpret_cast<char*>(pool);
+  p.table = table; p.refs = refcounts; p.new_table = new_table; p.new_refs = new_refcounts; p.live = live;
+  p.nblk = (pages + kCompactPer - 1) / kCompactPer;
+  int32_t* w = reinterpret_cast<int32_t*>(workspace);
+  p.counts = w; w += up4(p.nblk + 1);
+  p.rank = w; w += up4(pages);
+  p.src = w; w += up4(pages);
+  p.dst = w;
+  p.table_row = table_row; p.page_bytes = page_bytes; p.rows = rows; p.slots = slots; p.pages = pages;
+  hipStream_t st = (hipStream_t)stream;
+  paged_compact_count_kernel<<<p.nblk, 1024, 0, st>>>(p);
+  if (int rc = launch_status("paged_compact count")) return rc;
+  paged_compact_plan_kernel<<<p.nblk, 1024, 0, st>>>(p);
+  if (int rc = launch_status("paged_compact plan")) return rc;
+  paged_compact_apply_kernel<<<2048, 256, 0, st>>>(p, page_bytes / 16);
+  return launch_status("paged_compact");
+}

@@ -1,0 +1,186 @@
+"""Host side of the decoding operators, on the CPU: argument checks of the C-ABI and of the wrappers, the page arithmetic, and the oracle itself."""
+import ctypes as C
+import math
+import subprocess
+from pathlib import Path
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import decoding_oracle as od
+
+ROOT = Path(__file__).resolve().parents[1]
+
+
+@pytest.fixture(scope="module")
+def L():
+    from multimodal_amd import _lib, build
+
+    build.build()
+    return _lib.lib()
+
+
+def cache(**kw):
+    from multimodal_amd.ops import _PagedCache
+
+    d = dict(key_pages=4096, value_pages=8192, page_table=64, key_page_stride=2048, key_head_stride=1024, key_token_stride=64, value_page_stride=2048,
+             value_head_stride=1024, value_token_stride=64, table_row_stride=4, dtype=1, pages=8, page_size=16, slots=4, kv_heads=2, dim=64)
+    d.update(kw)
+    return _PagedCache(**d)
+
+
+def attention(L, c, lengths=64, q=256, k=None, v=None, out=256, rows=1, heads=2, q_row=128, ws=None, bytes_=0):
+    return L.mmamd_paged_attention(C.byref(c) if c is not None else None, lengths, q, q_row, 64, k, 64, 64, v, 64, 64, out, rows, heads, 0.125, ws, bytes_, None)
+
+
+def test_attention_arguments(L):
+    """Every refusal comes before a launch, with a message (addresses here are no memory)."""
+    assert attention(L, None) == -1 and b"null cache" in L.mmamd_last_error()
+    for kw, code in [(dict(key_pages=None), -1), (dict(page_table=None), -1), (dict(dtype=2), -2), (dict(pages=0), -1), (dict(page_size=0), -1), (dict(slots=-1), -1),
+                     (dict(kv_heads=0), -1), (dict(dim=80), -2), (dict(key_pages=4104), -3), (dict(key_token_stride=60), -3), (dict(value_head_stride=-64), -3),
+                     (dict(slots=1 << 26, page_size=32), -2)]:
+        assert attention(L, cache(**kw)) == code, kw
+        assert L.mmamd_paged_attention_workspace(C.byref(cache(**kw)), 1, 2) == code, kw
+        assert L.mmamd_paged_append(C.byref(cache(**kw)), 256, 64, 64, 64, 256, 64, 64, 64, 64, None, 1, 1, None) == code, kw
+    c = cache()
+    assert attention(L, c, heads=3) == -1 and attention(L, c, rows=-1) == -1 and attention(L, c, rows=70000) == -2
+    assert attention(L, c, q=None) == -1 and attention(L, c, lengths=None) == -1 and attention(L, c, out=None) == -1
+    assert attention(L, c, k=256) == -1 and b"one of k and v" in L.mmamd_last_error()
+    assert attention(L, c, q=258) == -3 and attention(L, c, q_row=65) == -3
+    big = cache(slots=1000)
+    need = L.mmamd_paged_attention_workspace(C.byref(big), 1, 2)
+    assert need > 0 and attention(L, big, ws=None, bytes_=need) == -1 and attention(L, big, ws=256, bytes_=need - 1) == -1
+    assert b"needed" in L.mmamd_last_error()
+    assert attention(L, c, rows=0) == 0  # nothing to do
+    assert L.mmamd_paged_append(C.byref(c), 256, 64, 64, 64, 256, 64, 64, 64, None, None, 1, 1, None) == -1
+    assert L.mmamd_paged_append(C.byref(c), 256, 64, 60, 64, 256, 64, 64, 64, 64, None, 1, 1, None) == -3
+    assert L.mmamd_paged_append(C.byref(c), 256, 64, 64, 64, 256, 64, 64, 64, 64, None, 1, 1 << 28, None) == -2
+    assert L.mmamd_paged_append(C.byref(c), None, 64, 64, 64, None, 64, 64, 64, None, None, 0, 4, None) == 0
+
+
+def test_fork_compact_and_beam_arguments(L):
+    def fork(pool=4096, pages=8, blocks=2, page=16, row=128, table=64, lengths=64, refs=64, old=2, slots=4, parents=64, rows=2, new=64, ws=256, size=1 << 20):
+        return L.mmamd_paged_fork(pool, pages, blocks, page, row, table, slots, lengths, refs, old, slots, parents, rows, None, 1, new, new, new, new, ws, size, None)
+
+    for kw, code in [(dict(pages=0), -1), (dict(blocks=0), -1), (dict(slots=0), -1), (dict(rows=-1), -1), (dict(pool=None), -1), (dict(refs=None), -1), (dict(table=None), -1),
+                     (dict(parents=None), -1), (dict(ws=None), -1), (dict(size=8), -1), (dict(row=120), -3), (dict(pool=4100), -3), (dict(rows=65534), -2),
+                     (dict(slots=1 << 27), -2)]:
+        assert fork(**kw) == code, kw
+    assert L.mmamd_paged_fork_workspace(2, 2, 0, 8) == -1 and L.mmamd_paged_fork_workspace(2, 3, 4, 8) > 0
+
+    def compact(pool=4096, pages=8, size=4096, table=64, rows=2, slots=4, refs=64, new=64, ws=256, bytes_=1 << 20):
+        return L.mmamd_paged_compact(pool, pages, size, table, slots, rows, slots, refs, new, new, new, ws, bytes_, None)
+
+    for kw, code in [(dict(pages=0), -1), (dict(size=0), -1), (dict(size=100), -3), (dict(pool=None), -1), (dict(table=None), -1), (dict(ws=None), -1), (dict(bytes_=4), -1)]:
+        assert compact(**kw) == code, kw
+
+    def beam(logits=256, dtype=0, ld=100, scores=64, seq=None, out=64, out_seq=None, tokens=0, eos=3, penalty=0.0, groups=1, beams=4, vocab=100, ws=256, size=1 << 20):
+        return L.mmamd_beam_search_step(logits, dtype, ld, scores, 64, 64, seq, tokens, eos, penalty, groups, beams, vocab, out, 64, 64, 64, 64, out_seq, ws, size, None)
+
+    for kw, code in [(dict(logits=None), -1), (dict(dtype=3), -2), (dict(beams=33), -2), (dict(beams=0), -1), (dict(groups=30000), -2), (dict(vocab=0), -1), (dict(eos=100), -1),
+                     (dict(eos=-1), -1), (dict(seq=64), -1), (dict(penalty=math.nan), -1), (dict(size=4), -1), (dict(ws=None), -1), (dict(out=None), -1), (dict(ld=-1), -1)]:
+        assert beam(**kw) == code, kw
+    assert beam(groups=0) == 0
+
+
+def test_wrappers_refuse_host_tensors_and_wrong_types():
+    from multimodal_amd import ops
+
+    q, pages, table, n = torch.zeros(1, 2, 64), torch.zeros(4, 2, 16, 64), torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
+    with pytest.raises(ops.MmamdError, match="no CPU fallback"):
+        ops.paged_attention(q, pages, pages, table, n)
+    with pytest.raises(ops.MmamdError, match="float32 or bfloat16"):
+        ops.paged_attention(q, pages.half(), pages.half(), table, n)
+    with pytest.raises(ops.MmamdError, match="tensor"):
+        ops.paged_attention(q[0], pages, pages, table, n)
+    with pytest.raises(ops.MmamdError, match="no CPU fallback"):
+        ops.paged_append(q[None], q[None], pages, pages, table, n)
+    with pytest.raises(ops.MmamdError, match="no CPU fallback"):
+        ops.paged_fork(pages, table, n, n, n)
+    with pytest.raises(ops.MmamdError, match="no CPU fallback"):
+        ops.paged_compact(pages, table, n)
+    with pytest.raises(ops.MmamdError, match="no CPU fallback"):
+        ops.beam_search_step(torch.zeros(2, 5), torch.zeros(1, 2), table, table.bool(), None, 0)
+    with pytest.raises(ops.MmamdError, match="float32 or bfloat16"):
+        ops.beam_search_step(torch.zeros(2, 5).double(), torch.zeros(1, 2), table, table.bool(), None, 0)
+
+
+def test_page_division(tmp_path):
+    """div_by (csrc/paged.h) is the division, for every divisor and the numerators around its multiples."""
+    from multimodal_amd import build
+
+    (tmp_path / "e.hip").write_text("namespace mmamd { void set_error(const char*, ...) {} void count_launch(const char*) {} }")
+    (tmp_path / "t.hip").write_text(f'''
+#include "{ROOT}/multimodal_amd/csrc/paged.h"
+int main() {{
+  for (uint32_t d = 1; d < 70000; d = d < 300 ? d + 1 : d * 1.37) {{
+    const mmamd::FastDiv f = mmamd::fast_div(d);
+    for (uint64_t k = 0; k * d < 0xffffffffull; k = k < 100 ? k + 1 : k * 1.1 + 1)
+      for (int64_t e = -1; e <= 1; ++e) {{
+        const int64_t n = (int64_t)(k * d) + e;
+        if (n >= 0 && n <= 0xffffffffll && mmamd::div_by(f, (uint32_t)n) != (uint32_t)n / d) return 1;
+      }}
+    if (mmamd::div_by(f, 0xffffffffu) != 0xffffffffu / d) return 2;
+  }}
+  return 0;
+}}''')
+    subprocess.run([build._hipcc(), "-O1", "-std=c++17", "--offload-arch=gfx950", "--offload-host-only", "-Wno-return-type", str(tmp_path / "t.hip"), str(tmp_path / "e.hip"),
+                    "-o", str(tmp_path / "t")], check=True, capture_output=True)
+    assert subprocess.run([str(tmp_path / "t")]).returncode == 0
+
+
+def test_oracle_attention_equals_dense():
+    """Pages in order and out of order give what one dense softmax gives; bad pages are as if their tokens were not there."""
+    rng = np.random.default_rng(0)
+    kp, vp = rng.standard_normal((2, 6, 2, 4, 8))
+    q = rng.standard_normal((2, 4, 8))
+    table = np.array([[3, 0, 5], [1, 9, 2]], np.int32)
+    out, kp2, _, _ = od.paged_attention(q, kp, vp, table, np.array([10, 12]))
+    np.testing.assert_array_equal(kp, kp2)
+    for r, ids in ((0, [3, 0, 5]), (1, [1, 2])):
+        n = 10 if r == 0 else 8
+        for h in range(4):
+            kk, vv = (np.concatenate([x[i, h // 2] for i in ids])[:n] for x in (kp, vp))
+            s = kk @ q[r, h] / math.sqrt(8)
+            w = np.exp(s - s.max())
+            np.testing.assert_allclose(out[r, h], w @ vv / w.sum(), atol=1e-12)
+    out, kp2, vp2, _ = od.paged_attention(q, kp, vp, table, np.array([10, 4]), kp[0, :, :2].transpose(1, 0, 2), vp[0, :, :2].transpose(1, 0, 2))
+    np.testing.assert_array_equal(kp2[5, :, 2], kp[0, :, 0])  # position 10 = place 2 of page 5
+    np.testing.assert_array_equal(np.delete(kp2, 5, 0), np.delete(kp, 5, 0))  # position 4 of the second row lies on page 9, which is none
+    assert not od.paged_attention(q, kp, vp, table, np.array([0, -3]))[0].any()
+
+
+def test_oracle_fork_keeps_counts():
+    rng = np.random.default_rng(1)
+    pool = rng.standard_normal((40, 2, 4, 8))
+    table, lengths, refs = np.full((0, 6), -1, np.int32), np.zeros(0, np.int32), np.zeros(40, np.int32)
+    pool, table, lengths, refs, short = od.paged_fork(pool, table, lengths, refs, [-1, -1], [5, 9])
+    lengths = np.array([5, 9])
+    for step in range(8):
+        parents = rng.integers(0, len(lengths), 4)
+        tokens = [[pool[table[p, t // 4]][..., t % 4, :].copy() for t in range(lengths[p])] for p in parents]
+        pool, table, lengths, refs, short = od.paged_fork(pool, table, lengths, refs, parents, 1)
+        assert short == 0
+        np.testing.assert_array_equal(np.bincount(table[table >= 0], minlength=40), refs)
+        for r, row in enumerate(tokens):
+            for t, x in enumerate(row):
+                np.testing.assert_array_equal(pool[table[r, t // 4]][..., t % 4, :], x)
+        pool, table, refs, live = od.paged_compact(pool, table, refs)
+        assert (refs[:live] > 0).all() and not refs[live:].any()
+        for r in range(4):  # a new token of its own for every row
+            pool[table[r, lengths[r] // 4]][..., lengths[r] % 4, :] = rng.standard_normal((2, 8))
+        lengths = lengths + 1
+
+
+def test_oracle_beam_equals_sort():
+    rng = np.random.default_rng(2)
+    logits, scores = rng.standard_normal((6, 11)), -rng.random((2, 3)).cumsum(1)
+    res = od.beam_search_step(logits, scores, np.full((2, 3), 4), np.zeros((2, 3), bool), None, 0)
+    logp = logits - np.log(np.exp(logits).sum(1, keepdims=True))
+    for g in range(2):
+        flat = (scores[g][:, None] + logp[3 * g:3 * g + 3]).ravel()
+        best = np.argsort(-flat)[:3]
+        np.testing.assert_allclose(res[0][g], flat[best])
+        np.testing.assert_array_equal(res[3][g], best % 11)
+        np.testing.assert_array_equal(res[4][g], best // 11 + 3 * g)
