@@ -22,26 +22,6 @@ struct PagedAttnParams {
   float scale_log2e;
 };
 
-// 16 bytes of T as floats
-template <typename T>
-struct Vec16;
-template <>
-struct Vec16<float> {
-  static constexpr int N = 4;
-  static __device__ __forceinline__ void unpack(const uint4& u, float (&f)[4]) {
-    f[0] = __uint_as_float(u.x); f[1] = __uint_as_float(u.y); f[2] = __uint_as_float(u.z); f[3] = __uint_as_float(u.w);
-  }
-};
-template <>
-struct Vec16<bf16> {
-  static constexpr int N = 8;
-  static __device__ __forceinline__ void unpack(const uint4& u, float (&f)[8]) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { f[2 * i] = __uint_as_float(w[i] << 16); f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-  }
-};
-
 // the tokens [begin, end) of a row that split s of it takes; chunks of at least min_chunk tokens, so that a short row is not cut up.  Every kernel
 // that needs to know which splits of a row hold anything asks here.
 __device__ __forceinline__ int row_chunk(const PagedAttnParams& p, int n) {
@@ -57,183 +37,266 @@ __device__ __forceinline__ int row_tokens(const PagedAttnParams& p, int row, int
   return pos >= 0 ? len + 1 : clamp_int(len, 0, cap);
 }
 
-// One workgroup: GT query heads of one key head of one row over one split of the row's tokens.  Four lanes share a token (each a quarter of its
-// dims, in 16-byte pieces), a wave has 16 tokens in flight per step and U steps at once; every lane group keeps the running maximum, sum and output
-// of its own tokens in fp32, joined by shuffles at the end, the four waves through LDS, the splits by paged_join_kernel.
-template <typename T, int D, int GT, int U>
-__global__ __launch_bounds__(256) void paged_attn_kernel(const PagedAttnParams p) {
-  constexpr int EV = Vec16<T>::N;               // values per 16 bytes
-  constexpr int NV = D / (4 * EV);              // 16-byte pieces per lane and token
-  constexpr int DL = NV * EV;                   // values per lane and token
+// LDS transpose read: within each 16-lane group, lane i points at 4 contiguous 16-bit values -- row i >> 2, columns 4 (i & 3) .. + 3 of a [4][16] block --
+// and receives column i of the block.
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+__device__ __forceinline__ s16x4 lds_columns(const bf16* at) { return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at); }
+
+template <typename T>
+__device__ __forceinline__ f32x4 mma16(const uint4& a, const uint4& b, f32x4 c);  // c += a b over the 4 pieces of 16 bytes that 4 lanes hold of a row
+template <>
+__device__ __forceinline__ f32x4 mma16<bf16>(const uint4& a, const uint4& b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x4 mma16<float>(const uint4& a, const uint4& b, f32x4 c) {
+  const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], c, 0, 0, 0);
+  return c;
+}
+
+// One workgroup: up to 16 query heads of one key head of one row over one split of the row's tokens, so that the cache is read once whatever the group
+// is.  The four waves take the split's tiles (32 tokens in bf16, 16 in fp32) in turn, each with its own running maximum, sum and output:
+//   scores [token, head] = K . q: the tile's keys go from memory to the registers of a 16 x 16 product as they lie (lane = token, 4 lanes share a row);
+//   out [dim, head] += V^T . weights: the values go through LDS for their columns, the weights are where the first product left them.
+// A pass over a tile ends with the loads of the next one in flight, and the page numbers of the one after.  fp32 runs on the fp32 matrix instruction.
+// bf16 weights are split in two bf16 parts (2^-16 of a weight is lost): in one part they would lose as much as the output's own rounding.
+template <typename T, int D>
+__global__ __launch_bounds__(256, 2) void paged_attn_kernel(const PagedAttnParams p) {
+  constexpr int TOK = sizeof(T) == 2 ? 32 : 16;      // tokens of a tile
+  constexpr int NT = TOK / 16;
+  constexpr int PIECES = D * (int)sizeof(T) / 16;    // 16-byte pieces of a row
+  constexpr int KP = PIECES / 4, VP = TOK * PIECES / 64;
+  constexpr int VROW = D + 16 / (int)sizeof(T);      // row of the values in LDS: the odd 16 bytes spread 16 rows over the banks
+  constexpr int ND = D / 16;
+  constexpr int RROW = D + 4;
+  constexpr int VBYTES = TOK * VROW * (int)sizeof(T), RBYTES = 16 * RROW * 4;
+  __shared__ __attribute__((aligned(16))) char smem[4 * (VBYTES > RBYTES ? VBYTES : RBYTES)];
+  __shared__ float red_m[4][16], red_l[4][16];
+
   const int row = blockIdx.z, kvh = blockIdx.y / p.sub, sg = blockIdx.y - kvh * p.sub, split = blockIdx.x;
   int pos;
   const int n = row_tokens(p, row, pos);
   const int chunk = row_chunk(p, n);
   const int begin = split * chunk, end = (begin + chunk < n) ? begin + chunk : n;
-  if (begin >= n && !(split == 0)) return;      // (split 0 of an empty row writes its zeros)
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = lane & 3, quad = lane >> 2;
-  const int h0 = kvh * p.group + sg * GT;
-  const int nh = (p.group - sg * GT) < GT ? (p.group - sg * GT) : GT;
+  if (begin >= n && split != 0) return;              // (split 0 of an empty row writes its zeros)
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l15 = lane & 15, quarter = lane >> 4;
+  const int h0 = kvh * p.group + sg * 16;
+  const int nh = (p.group - sg * 16) < 16 ? (p.group - sg * 16) : 16;
+  T* vs = reinterpret_cast<T*>(smem + wave * VBYTES);
 
-  float q[GT][DL];
+  uint4 qf[KP];
+  {
+    const T* qp = reinterpret_cast<const T*>(p.q) + row * p.q_row + (h0 + (l15 < nh ? l15 : 0)) * p.q_head;
 #pragma unroll
-  for (int g = 0; g < GT; ++g) {
-    const T* qp = reinterpret_cast<const T*>(p.q) + row * p.q_row + (h0 + (g < nh ? g : 0)) * p.q_head;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      float f[EV];
-      Vec16<T>::unpack(*reinterpret_cast<const uint4*>(qp + (i * 4 + c) * EV), f);
-#pragma unroll
-      for (int e = 0; e < EV; ++e) q[g][i * EV + e] = f[e] * p.scale_log2e;
-    }
-  }
-  float m[GT], l[GT], o[GT][DL];
-#pragma unroll
-  for (int g = 0; g < GT; ++g) {
-    m[g] = -3.402823466e38f;
-    l[g] = 0.f;
-#pragma unroll
-    for (int e = 0; e < DL; ++e) o[g][e] = 0.f;
+    for (int i = 0; i < KP; ++i) qf[i] = reinterpret_cast<const uint4*>(qp)[i * 4 + quarter];
   }
   const int32_t* table = p.table + row * p.table_row;
-  const T* keys = reinterpret_cast<const T*>(p.keys) + kvh * p.key_head;
-  const T* values = reinterpret_cast<const T*>(p.values) + kvh * p.value_head;
-  const T* knew = reinterpret_cast<const T*>(p.k) + row * p.k_row + kvh * p.k_head;
-  const T* vnew = reinterpret_cast<const T*>(p.v) + row * p.v_row + kvh * p.v_head;
+  char* const keys = reinterpret_cast<char*>(p.keys) + kvh * p.key_head * (int64_t)sizeof(T);
+  char* const values = reinterpret_cast<char*>(p.values) + kvh * p.value_head * (int64_t)sizeof(T);
+  const char* const knew = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.k) + row * p.k_row + kvh * p.k_head);
+  const char* const vnew = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.v) + row * p.v_row + kvh * p.v_head);
 
-  for (int t0 = begin + wave * 16 * U; t0 < end; t0 += 4 * 16 * U) {
-    uint4 kr[U][NV], vr[U][NV];
-    bool ok[U];
+  uint4 kr[NT][KP], vr[VP];
+  uint32_t okmask = 0;                               // which tokens of the loaded tile take part
+  auto page_of = [&](int t0) {                       // page number of token t0 + lane % TOK; -1 behind the split's end
+    const int t = t0 + (lane & (TOK - 1));
+    const int id = t < end ? table[div_by(p.page, (uint32_t)t)] : -1;
+    return (uint32_t)id < (uint32_t)p.pages ? id : -1;
+  };
+  auto load_tile = [&](int t0, int id) {
+    const int t = t0 + (lane & (TOK - 1));
+    okmask = (uint32_t)__ballot(id >= 0 && lane < TOK);
+    const int off = t - (int)(div_by(p.page, (uint32_t)t) * p.page.d);
+    const int64_t pg = id >= 0 ? id : 0;             // a place that holds no token is read as page 0, which exists, and not used
+    int64_t ko = (pg * p.key_page + off * p.key_token) * (int64_t)sizeof(T), vo = (pg * p.value_page + off * p.value_token) * (int64_t)sizeof(T);
+    if (id >= 0 && t == pos) { ko = knew - keys; vo = vnew - values; }
+    const int klo = (int)ko, khi = (int)(ko >> 32), vlo = (int)vo, vhi = (int)(vo >> 32);
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int t = t0 + u * 16 + quad;
-      const int tc = t < end ? t : end - 1;                     // loads never leave the row
-      const int slot = (int)div_by(p.page, (uint32_t)tc), off = tc - slot * (int)p.page.d;
-      const int id = table[slot];
-      const bool inside = (uint32_t)id < (uint32_t)p.pages;
-      ok[u] = inside && t < end;
-      const int64_t pg = inside ? id : 0;
-      T* kp = const_cast<T*>(keys) + pg * p.key_page + off * p.key_token;
-      T* vp = const_cast<T*>(values) + pg * p.value_page + off * p.value_token;
-      const bool fresh = t == pos;
-      const T* ks = fresh ? knew : kp;
-      const T* vs = fresh ? vnew : vp;
+    for (int u = 0; u < NT; ++u) {
+      const int64_t o = (int64_t)(((uint64_t)(uint32_t)__shfl(khi, u * 16 + l15) << 32) | (uint32_t)__shfl(klo, u * 16 + l15));
 #pragma unroll
-      for (int i = 0; i < NV; ++i) kr[u][i] = *reinterpret_cast<const uint4*>(ks + (i * 4 + c) * EV);
-#pragma unroll
-      for (int i = 0; i < NV; ++i) vr[u][i] = *reinterpret_cast<const uint4*>(vs + (i * 4 + c) * EV);
-      if (fresh && ok[u] && sg == 0) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          *reinterpret_cast<uint4*>(kp + (i * 4 + c) * EV) = kr[u][i];
-          *reinterpret_cast<uint4*>(vp + (i * 4 + c) * EV) = vr[u][i];
-        }
-      }
-      if (!ok[u]) {  // what lies in a place that holds no token may be anything, NaN too
-#pragma unroll
-        for (int i = 0; i < NV; ++i) vr[u][i] = make_uint4(0, 0, 0, 0);
-      }
+      for (int i = 0; i < KP; ++i) kr[u][i] = *reinterpret_cast<const uint4*>(keys + o + (i * 4 + quarter) * 16);
     }
 #pragma unroll
-    for (int g = 0; g < GT; ++g) {
-      float s[U], top = m[g];
+    for (int i = 0; i < VP; ++i) {
+      const int piece = i * 64 + lane, tok = piece / PIECES, x = piece - tok * PIECES;
+      const int64_t o = (int64_t)(((uint64_t)(uint32_t)__shfl(vhi, tok) << 32) | (uint32_t)__shfl(vlo, tok));
+      vr[i] = *reinterpret_cast<const uint4*>(values + o + x * 16);
+    }
+  };
+
+  float m = -3.402823466e38f, l = 0.f;
+  f32x4 o[ND];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float a = 0.f;
+  for (int d = 0; d < ND; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+  int t0 = begin + wave * TOK;
+  int id = page_of(t0);
+  if (t0 < end) load_tile(t0, id);
+  id = page_of(t0 + 4 * TOK);
+  for (; t0 < end; t0 += 4 * TOK) {
+    const uint32_t ok = okmask;
+    if (pos >= t0 && pos < t0 + TOK && sg == 0 && (ok >> (pos - t0) & 1u)) {  // the new token into its place
+      const int slot = (int)div_by(p.page, (uint32_t)pos), off = pos - slot * (int)p.page.d;
+      const int64_t pg = table[slot];
+      char* kd = keys + (pg * p.key_page + off * p.key_token) * (int64_t)sizeof(T);
+      char* vd = values + (pg * p.value_page + off * p.value_token) * (int64_t)sizeof(T);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          float f[EV];
-          Vec16<T>::unpack(kr[u][i], f);
+      for (int u = 0; u < NT; ++u)
+        if (t0 + u * 16 + l15 == pos) {
 #pragma unroll
-          for (int e = 0; e < EV; ++e) a = fmaf(q[g][i * EV + e], f[e], a);
+          for (int i = 0; i < KP; ++i) *reinterpret_cast<uint4*>(kd + (i * 4 + quarter) * 16) = kr[u][i];
         }
-        a += __shfl_xor(a, 1);
-        a += __shfl_xor(a, 2);
-        s[u] = ok[u] ? a : -INFINITY;
-        top = fmaxf(top, s[u]);
-      }
-      const float fac = __builtin_amdgcn_exp2f(m[g] - top);
-      m[g] = top;
-      l[g] *= fac;
 #pragma unroll
-      for (int e = 0; e < DL; ++e) o[g][e] *= fac;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const float w = __builtin_amdgcn_exp2f(s[u] - top);
-        l[g] += w;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-          float f[EV];
-          Vec16<T>::unpack(vr[u][i], f);
-#pragma unroll
-          for (int e = 0; e < EV; ++e) o[g][i * EV + e] = fmaf(w, f[e], o[g][i * EV + e]);
-        }
+      for (int i = 0; i < VP; ++i) {
+        const int piece = i * 64 + lane, tok = piece / PIECES, x = piece - tok * PIECES;
+        if (t0 + tok == pos) *reinterpret_cast<uint4*>(vd + x * 16) = vr[i];
       }
     }
+    f32x4 s[NT];
+#pragma unroll
+    for (int u = 0; u < NT; ++u) {
+      s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < KP; ++i) s[u] = mma16<T>(kr[u][i], qf[i], s[u]);
+    }
+    const bool whole = ok == (TOK == 32 ? 0xffffffffu : 0xffffu);
+#pragma unroll
+    for (int i = 0; i < VP; ++i) {
+      const int piece = i * 64 + lane, tok = piece / PIECES, x = piece - tok * PIECES;
+      if (!whole && !(ok >> tok & 1u)) vr[i] = make_uint4(0, 0, 0, 0);  // what lies where no token is may be anything, NaN too
+      *reinterpret_cast<uint4*>(vs + tok * VROW + x * (16 / (int)sizeof(T))) = vr[i];
+    }
+    if (t0 + 4 * TOK < end) {
+      load_tile(t0 + 4 * TOK, id);
+      id = page_of(t0 + 8 * TOK);
+    }
+    // weights: this lane has head l15 and the tokens u * 16 + 4 quarter + i
+    float top = m;
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[u][i] = (ok >> (u * 16 + quarter * 4 + i) & 1u) ? s[u][i] * p.scale_log2e : -INFINITY;
+        top = fmaxf(top, s[u][i]);
+      }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    const float fac = __builtin_amdgcn_exp2f(m - top);
+    m = top;
+    l *= fac;
+#pragma unroll
+    for (int d = 0; d < ND; ++d) o[d] *= fac;
+#pragma unroll
+    for (int u = 0; u < NT; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[u][i] = __builtin_amdgcn_exp2f(s[u][i] - top);
+        l += s[u][i];
+      }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's values are in LDS
+    if constexpr (sizeof(T) == 2) {
+      bf16x8 hi, lo;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          hi[u * 4 + i] = (bf16)s[u][i];
+          lo[u * 4 + i] = (bf16)(s[u][i] - (float)hi[u * 4 + i]);
+        }
+#pragma unroll
+      for (int d = 0; d < ND; ++d) {
+        const bf16* at = reinterpret_cast<const bf16*>(vs) + (quarter * 4 + (l15 >> 2)) * VROW + d * 16 + (l15 & 3) * 4;
+        const s16x4 a0 = lds_columns(at), a1 = lds_columns(at + 16 * VROW);
+        typedef __attribute__((ext_vector_type(8))) short s16x8;
+        const bf16x8 a = __builtin_bit_cast(bf16x8, (s16x8)__builtin_shufflevector(a0, a1, 0, 1, 2, 3, 4, 5, 6, 7));
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, hi, o[d], 0, 0, 0);
+        o[d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, lo, o[d], 0, 0, 0);
+      }
+    } else {
+#pragma unroll
+      for (int d = 0; d < ND; ++d)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[d] = __builtin_amdgcn_mfma_f32_16x16x4f32(reinterpret_cast<const float*>(vs)[(quarter * 4 + i) * VROW + d * 16 + l15], s[0][i], o[d], 0, 0, 0);
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // ... and read, before the next tile's overwrite them
   }
-  // join the 16 lane groups of the wave, then the four waves
-  __shared__ float red[4][GT][D + 2];
+  // join the four waves
+  l += __shfl_xor(l, 16);
+  l += __shfl_xor(l, 32);
+  __syncthreads();
+  float* const red = reinterpret_cast<float*>(smem);
+  if (l15 < nh) {
+    float* r = red + (wave * 16 + l15) * RROW + quarter * 4;
 #pragma unroll
-  for (int g = 0; g < GT; ++g) {
-    float top = m[g];
-#pragma unroll
-    for (int x = 4; x < 64; x <<= 1) top = fmaxf(top, __shfl_xor(top, x));
-    const float fac = __builtin_amdgcn_exp2f(m[g] - top);
-    float ls = l[g] * fac;
-#pragma unroll
-    for (int x = 4; x < 64; x <<= 1) ls += __shfl_xor(ls, x);
-#pragma unroll
-    for (int e = 0; e < DL; ++e) {
-      float v = o[g][e] * fac;
-#pragma unroll
-      for (int x = 4; x < 64; x <<= 1) v += __shfl_xor(v, x);
-      if (quad == 0) red[wave][g][((e / EV) * 4 + c) * EV + e % EV] = v;
-    }
-    if (lane == 0) { red[wave][g][D] = top; red[wave][g][D + 1] = ls; }
+    for (int d = 0; d < ND; ++d) *reinterpret_cast<f32x4*>(r + d * 16) = o[d];
+    if (quarter == 0) { red_m[wave][l15] = m; red_l[wave][l15] = l; }
   }
   __syncthreads();
   for (int i = threadIdx.x; i < nh * D; i += 256) {
     const int g = i / D, d = i - g * D;
-    float top = red[0][g][D];
+    float top = red_m[0][g];
 #pragma unroll
-    for (int w = 1; w < 4; ++w) top = fmaxf(top, red[w][g][D]);
+    for (int w = 1; w < 4; ++w) top = fmaxf(top, red_m[w][g]);
     float ls = 0.f, v = 0.f;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {
-      const float fac = __builtin_amdgcn_exp2f(red[w][g][D] - top);
-      ls = fmaf(red[w][g][D + 1], fac, ls);
-      v = fmaf(red[w][g][d], fac, v);
+      const float fac = __builtin_amdgcn_exp2f(red_m[w][g] - top);
+      ls = fmaf(red_l[w][g], fac, ls);
+      v = fmaf(red[(w * 16 + g) * RROW + d], fac, v);
     }
     const int64_t rh = (int64_t)row * p.heads + h0 + g;
     if (p.splits == 1) {
       reinterpret_cast<T*>(p.out)[rh * D + d] = (T)(ls == 0.f ? 0.f : v / ls);
     } else {
-      float* w = p.ws + (rh * p.splits + split) * (D + 2);
-      w[d] = v;
-      if (d == 0) { w[D] = top; w[D + 1] = ls; }
+      const int64_t at = rh * p.splits + split;
+      p.ws[at * D + d] = v;
+      if (d == 0) reinterpret_cast<float2*>(p.ws + (int64_t)p.rows * p.heads * p.splits * D)[at] = make_float2(top, ls);
     }
   }
 }
 
-// Joins the splits of a (row, head): o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.
+// Joins the splits of a (row, head): o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  The statistics of all splits first, one a thread; then the
+// outputs, each group of D threads every NG-th split, whose loads do not wait for one another.
+constexpr int kSplitsMost = 256;
 template <typename T, int D>
-__global__ __launch_bounds__(D) void paged_join_kernel(const PagedAttnParams p) {
-  const int h = blockIdx.x, row = blockIdx.y, d = threadIdx.x;
+__global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p) {
+  constexpr int NG = 256 / D;
+  __shared__ float w[kSplitsMost], part[NG][D], red[4], sums[4];
+  const int h = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int pos;
   const int n = row_tokens(p, row, pos);
   const int chunk = row_chunk(p, n);
   const int used = n > 0 ? (n + chunk - 1) / chunk : 1;
   const int64_t rh = (int64_t)row * p.heads + h;
-  const float* w = p.ws + rh * p.splits * (D + 2);
-  float top = -3.402823466e38f, ls = 0.f, v = 0.f;
-  for (int s = 0; s < used; ++s, w += D + 2) {
-    const float ms = w[D], nt = fmaxf(top, ms);
-    const float fa = __builtin_amdgcn_exp2f(top - nt), fb = __builtin_amdgcn_exp2f(ms - nt);
-    ls = ls * fa + w[D + 1] * fb;
-    v = v * fa + w[d] * fb;
-    top = nt;
+  const float2 ml = tid < used ? reinterpret_cast<const float2*>(p.ws + (int64_t)p.rows * p.heads * p.splits * D)[rh * p.splits + tid] : make_float2(-3.402823466e38f, 0.f);
+  float top = wave_max(ml.x);
+  if (lane == 0) red[wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  const float f = __builtin_amdgcn_exp2f(ml.x - top);
+  w[tid] = tid < used ? f : 0.f;
+  const float ls = wave_sum(ml.y * f);
+  if (lane == 0) sums[wave] = ls;
+  __syncthreads();
+  const int g = tid / D, d = tid - g * D;
+  if (g < NG) {
+    const float* o = p.ws + rh * p.splits * D + d;
+    float v = 0.f;
+#pragma unroll 8
+    for (int s = g; s < used; s += NG) v = fmaf(w[s], o[(int64_t)s * D], v);
+    part[g][d] = v;
   }
-  reinterpret_cast<T*>(p.out)[rh * D + d] = (T)(ls == 0.f ? 0.f : v / ls);
+  __syncthreads();
+  if (tid < D) {
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < NG; ++k) v += part[k][tid];
+    const float total = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    reinterpret_cast<T*>(p.out)[rh * D + tid] = (T)(total == 0.f ? 0.f : v / total);
+  }
 }
 
 // Splits of a row, from what the host knows: the rows, heads and the capacity of the page table (the lengths are on the device).
@@ -246,21 +309,18 @@ static int paged_splits(int rows, int heads, int kv_heads, int64_t capacity) {
   if (s > most) s = most;
   const int64_t grid = 16384 / wgs;
   if (s > grid) s = grid;
+  if (s > kSplitsMost) s = kSplitsMost;
   return s < 1 ? 1 : (int)s;
 }
 
 template <typename T, int D>
 static int launch_paged_attn(PagedAttnParams& p, hipStream_t st) {
-  constexpr int GT = 2;
-  const int gt = p.group == 1 ? 1 : GT;
-  p.sub = (p.group + gt - 1) / gt;
+  p.sub = (p.group + 15) / 16;
   p.min_chunk = 128;
-  const dim3 grid(p.splits, p.kv_heads * p.sub, p.rows);
-  if (gt == 1) paged_attn_kernel<T, D, 1, 2><<<grid, 256, 0, st>>>(p);
-  else paged_attn_kernel<T, D, GT, 2><<<grid, 256, 0, st>>>(p);
+  paged_attn_kernel<T, D><<<dim3(p.splits, p.kv_heads * p.sub, p.rows), 256, 0, st>>>(p);
   if (int rc = launch_status("paged_attention")) return rc;
   if (p.splits > 1) {
-    paged_join_kernel<T, D><<<dim3(p.heads, p.rows), D, 0, st>>>(p);
+    paged_join_kernel<T, D><<<dim3(p.heads, p.rows), 256, 0, st>>>(p);
     return launch_status("paged_attention join");
   }
   return 0;

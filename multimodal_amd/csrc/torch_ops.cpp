@@ -472,6 +472,200 @@ void clear_packed_impl() {
 
 }  // namespace
 
+namespace {
+
+// ---- decoding with a paged key-value cache (multimodal_amd/ops.py calls these: a decoding step is short, and its checks cost less here than in Python) ----
+using OptTensor = c10::optional<Tensor>;
+
+// one call's view of its tensors: all on the device of the first, which becomes the current one
+struct Checker {
+  const char* who;
+  at::Device device;
+  c10::hip::HIPGuardMasqueradingAsCUDA guard;
+  Checker(const char* w, const Tensor& t) : who(w), device(t.device()), guard(t.device()) {}
+  // -1 in `shape`: any size; contiguous in the last axis, or altogether where `whole`
+  void operator()(const Tensor& t, const char* name, at::ScalarType dt, at::IntArrayRef shape, bool whole = false) const {
+    TORCH_CHECK(t.is_cuda(), who, ": ", name, " is on ", t.device(), ": the MI355X path needs HIP device tensors (no CPU fallback)");
+    TORCH_CHECK(t.device() == device, who, ": ", name, " is on ", t.device(), ", the first tensor on ", device);
+    TORCH_CHECK(t.scalar_type() == dt, who, ": ", name, " must be ", dt, ", got ", t.scalar_type());
+    bool same = t.dim() == (int64_t)shape.size();
+    for (size_t i = 0; same && i < shape.size(); ++i) same = shape[i] < 0 || t.size(i) == shape[i];
+    TORCH_CHECK(same, who, ": ", name, " must have the shape ", shape, " (-1: any), got ", t.sizes());
+    TORCH_CHECK(t.numel() == 0 || (whole ? t.is_contiguous() : t.size(-1) <= 1 || t.stride(-1) == 1), who, ": ", name, " must be contiguous", whole ? "" : " in its last axis");
+    TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), who, " has no gradient (decoding): call it under torch.no_grad()");
+  }
+};
+// an axis of one entry is never stepped along, whatever its stride says
+int64_t step(const Tensor& t, int64_t axis) { return t.size(axis) > 1 ? t.stride(axis) : 0; }
+
+mmamd_paged_cache paged_cache(const Checker& ck, const Tensor& keys, const Tensor& values, const Tensor& table, int64_t rows) {
+  const at::ScalarType dt = keys.scalar_type();
+  TORCH_CHECK(dt == at::kFloat || dt == at::kBFloat16, ck.who, ": key_pages must be float32 or bfloat16, got ", dt);
+  ck(keys, "key_pages", dt, {-1, -1, -1, -1});
+  ck(values, "value_pages", dt, keys.sizes());
+  ck(table, "page_table", at::kInt, {rows, -1});
+  TORCH_CHECK(keys.numel() > 0 && table.size(1) > 0, ck.who, ": pages ", keys.sizes(), " and page_table ", table.sizes(), " must not be empty");
+  TORCH_CHECK(keys.size(0) < INT32_MAX && keys.size(2) < INT32_MAX && table.size(1) < INT32_MAX, ck.who, ": too many pages, tokens or slots");
+  mmamd_paged_cache c;
+  c.key_pages = keys.data_ptr(); c.value_pages = values.data_ptr(); c.page_table = (const int32_t*)table.data_ptr();
+  c.key_page_stride = step(keys, 0); c.key_head_stride = step(keys, 1); c.key_token_stride = step(keys, 2);
+  c.value_page_stride = step(values, 0); c.value_head_stride = step(values, 1); c.value_token_stride = step(values, 2);
+  c.table_row_stride = step(table, 0);
+  c.dtype = dt_code(dt); c.pages = (int32_t)keys.size(0); c.page_size = (int32_t)keys.size(2); c.slots = (int32_t)table.size(1);
+  c.kv_heads = (int32_t)keys.size(1); c.dim = (int32_t)keys.size(3);
+  return c;
+}
+
+Tensor workspace(int64_t bytes, const char* what, const Tensor& like) {
+  TORCH_CHECK(bytes >= 0, what, " failed (status ", bytes, "): ", mmamd_last_error());
+  return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor();
+}
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+int32_t* iptr(const Tensor& t) { return (int32_t*)ptr(t); }
+
+void paged_attention_into(const Tensor& q, const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& lengths, const OptTensor& k, const OptTensor& v,
+                          c10::optional<double> scale, const Tensor& out) {
+  const Checker ck("paged_attention", keys);
+  TORCH_CHECK(q.dim() == 3, "paged_attention: q must be a [rows, heads, dim] tensor");
+  const int64_t rows = q.size(0), heads = q.size(1);
+  const mmamd_paged_cache c = paged_cache(ck, keys, values, table, rows);
+  const at::ScalarType dt = keys.scalar_type();
+  ck(q, "q", dt, {rows, heads, c.dim});
+  ck(lengths, "lengths", at::kInt, {rows});
+  TORCH_CHECK(k.has_value() == v.has_value(), "paged_attention: k and v go together");
+  if (k.has_value()) {
+    ck(*k, "k", dt, {rows, c.kv_heads, c.dim});
+    ck(*v, "v", dt, {rows, c.kv_heads, c.dim});
+  }
+  ck(out, "out", dt, {rows, heads, c.dim}, true);
+  TORCH_CHECK(rows < INT32_MAX && heads < INT32_MAX, "paged_attention: too many rows or heads");
+  if (rows == 0) return;
+  const int64_t need = mmamd_paged_attention_workspace(&c, (int)rows, (int)heads);
+  const Tensor ws = workspace(need, "mmamd_paged_attention", q);
+  check_status(mmamd_paged_attention(&c, iptr(lengths), q.data_ptr(), step(q, 0), step(q, 1), k.has_value() ? k->data_ptr() : nullptr, k.has_value() ? step(*k, 0) : 0,
+                                     k.has_value() ? step(*k, 1) : 0, v.has_value() ? v->data_ptr() : nullptr, v.has_value() ? step(*v, 0) : 0, v.has_value() ? step(*v, 1) : 0,
+                                     out.data_ptr(), (int)rows, (int)heads, (float)(scale.has_value() ? *scale : 1.0 / std::sqrt((double)c.dim)), ptr(ws), need, cur_stream(q)),
+               "mmamd_paged_attention");
+}
+Tensor paged_attention_impl(const Tensor& q, const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& lengths, const OptTensor& k, const OptTensor& v,
+                            c10::optional<double> scale) {
+  Tensor out = at::empty(q.sizes(), q.options());
+  paged_attention_into(q, keys, values, table, lengths, k, v, scale, out);
+  return out;
+}
+Tensor paged_attention_meta(const Tensor& q, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, c10::optional<double>) {
+  return at::empty(q.sizes(), q.options());
+}
+void paged_attention_into_meta(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, c10::optional<double>, const Tensor&) {}
+
+void paged_append_impl(const Tensor& k, const Tensor& v, const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& start, const OptTensor& counts) {
+  const Checker ck("paged_append", keys);
+  TORCH_CHECK(k.dim() == 4, "paged_append: k must be a [rows, tokens, kv_heads, dim] tensor");
+  const int64_t rows = k.size(0), tokens = k.size(1);
+  const mmamd_paged_cache c = paged_cache(ck, keys, values, table, rows);
+  ck(k, "k", keys.scalar_type(), {rows, tokens, c.kv_heads, c.dim});
+  ck(v, "v", keys.scalar_type(), k.sizes());
+  ck(start, "start", at::kInt, {rows});
+  if (counts.has_value()) ck(*counts, "counts", at::kInt, {rows});
+  TORCH_CHECK(rows < INT32_MAX && tokens < INT32_MAX, "paged_append: too many rows or tokens");
+  if (k.numel() == 0) return;
+  check_status(mmamd_paged_append(&c, k.data_ptr(), step(k, 0), step(k, 1), step(k, 2), v.data_ptr(), step(v, 0), step(v, 1), step(v, 2), iptr(start),
+                                  counts.has_value() ? iptr(*counts) : nullptr, (int)rows, (int)tokens, cur_stream(k)),
+               "mmamd_paged_append");
+}
+void paged_append_meta(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptTensor&) {}
+
+void check_pool(const Checker& ck, const Tensor& pages, const Tensor& refcounts, const Tensor& table) {
+  TORCH_CHECK(pages.scalar_type() == at::kFloat || pages.scalar_type() == at::kBFloat16, ck.who, ": pages must be float32 or bfloat16, got ", pages.scalar_type());
+  TORCH_CHECK(pages.dim() >= 3, ck.who, ": pages must be a [pages, ..., page_size, dim] tensor, got ", pages.sizes());
+  ck(pages, "pages", pages.scalar_type(), pages.sizes(), true);
+  TORCH_CHECK(pages.numel() > 0 && pages.size(0) < INT32_MAX, ck.who, ": pages must not be empty, got ", pages.sizes());
+  ck(refcounts, "refcounts", at::kInt, {pages.size(0)});
+  ck(table, "page_table", at::kInt, {-1, -1});
+  TORCH_CHECK(table.size(1) > 0 && table.size(0) < INT32_MAX && table.size(1) < INT32_MAX, ck.who, ": page_table must have at least one slot, got ", table.sizes());
+}
+at::TensorOptions ints(const Tensor& t) { return t.options().dtype(at::kInt); }
+
+std::tuple<Tensor, Tensor, Tensor, Tensor> paged_fork_impl(const Tensor& pages, const Tensor& table, const Tensor& lengths, const Tensor& refcounts, const Tensor& parents,
+                                                           const OptTensor& reserve_rows, int64_t reserve) {
+  const Checker ck("paged_fork", pages);
+  check_pool(ck, pages, refcounts, table);
+  ck(lengths, "lengths", at::kInt, {table.size(0)});
+  ck(parents, "parents", at::kInt, {-1});
+  const int64_t old_rows = table.size(0), slots = table.size(1), rows = parents.size(0), n = pages.size(0), page = pages.size(-2), dim = pages.size(-1);
+  if (reserve_rows.has_value()) ck(*reserve_rows, "reserve", at::kInt, {rows});
+  TORCH_CHECK(reserve >= 0 && reserve <= INT32_MAX, "paged_fork: reserve must be a number of tokens, got ", reserve);
+  const int64_t blocks = pages.numel() / (n * page * dim);
+  TORCH_CHECK(rows < INT32_MAX && blocks < INT32_MAX && page < INT32_MAX, "paged_fork: too many rows, blocks or tokens");
+  Tensor new_table = at::empty({rows, slots}, ints(pages)), new_lengths = at::empty({rows}, ints(pages)), counts = at::empty({n}, ints(pages)), shortage = at::empty({1}, ints(pages));
+  const int64_t need = mmamd_paged_fork_workspace((int)old_rows, (int)rows, (int)slots, (int)n);
+  const Tensor ws = workspace(need, "mmamd_paged_fork", pages);
+  check_status(mmamd_paged_fork(pages.data_ptr(), (int)n, (int)blocks, (int)page, dim * (int64_t)pages.element_size(), iptr(table), step(table, 0), iptr(lengths), iptr(refcounts),
+                                (int)old_rows, (int)slots, iptr(parents), (int)rows, reserve_rows.has_value() ? iptr(*reserve_rows) : nullptr, (int)reserve, iptr(new_table),
+                                iptr(new_lengths), iptr(counts), iptr(shortage), ptr(ws), need, cur_stream(pages)),
+               "mmamd_paged_fork");
+  return {new_table, new_lengths, counts, shortage};
+}
+std::tuple<Tensor, Tensor, Tensor, Tensor> paged_fork_meta(const Tensor& pages, const Tensor& table, const Tensor&, const Tensor&, const Tensor& parents, const OptTensor&, int64_t) {
+  return {at::empty({parents.size(0), table.size(1)}, ints(pages)), at::empty({parents.size(0)}, ints(pages)), at::empty({pages.size(0)}, ints(pages)), at::empty({1}, ints(pages))};
+}
+
+std::tuple<Tensor, Tensor, Tensor> paged_compact_impl(const Tensor& pages, const Tensor& table, const Tensor& refcounts) {
+  const Checker ck("paged_compact", pages);
+  check_pool(ck, pages, refcounts, table);
+  const int64_t n = pages.size(0);
+  Tensor new_table = at::empty(table.sizes(), ints(pages)), counts = at::empty({n}, ints(pages)), live = at::empty({1}, ints(pages));
+  const int64_t need = mmamd_paged_compact_workspace((int)n);
+  const Tensor ws = workspace(need, "mmamd_paged_compact", pages);
+  check_status(mmamd_paged_compact(pages.data_ptr(), (int)n, pages.numel() / n * (int64_t)pages.element_size(), iptr(table), step(table, 0), (int)table.size(0), (int)table.size(1),
+                                   iptr(refcounts), iptr(new_table), iptr(counts), iptr(live), ptr(ws), need, cur_stream(pages)),
+               "mmamd_paged_compact");
+  return {new_table, counts, live};
+}
+std::tuple<Tensor, Tensor, Tensor> paged_compact_meta(const Tensor& pages, const Tensor& table, const Tensor&) {
+  return {at::empty(table.sizes(), ints(pages)), at::empty({pages.size(0)}, ints(pages)), at::empty({1}, ints(pages))};
+}
+
+using BeamOut = std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor>;
+BeamOut beam_outputs(const Tensor& scores, const OptTensor& sequences) {
+  const auto of = [&](at::ScalarType t) { return at::empty(scores.sizes(), scores.options().dtype(t)); };
+  return {of(at::kFloat), of(at::kInt), of(at::kBool), of(at::kLong), of(at::kInt),
+          sequences.has_value() ? at::empty(sequences->sizes(), sequences->options()) : at::empty({0}, scores.options().dtype(at::kLong))};
+}
+// (without sequences the last output is empty: the schema has no optional returns that every caller could unpack)
+BeamOut beam_search_step_impl(const Tensor& logits, const Tensor& scores, const Tensor& lengths, const Tensor& finished, const OptTensor& sequences, int64_t eos,
+                              double length_penalty) {
+  const Checker ck("beam_search_step", logits);
+  const at::ScalarType dt = logits.scalar_type();
+  TORCH_CHECK(dt == at::kFloat || dt == at::kBFloat16, "beam_search_step: logits must be float32 or bfloat16, got ", dt);
+  ck(scores, "scores", at::kFloat, {-1, -1}, true);
+  const int64_t groups = scores.size(0), beams = scores.size(1);
+  ck(logits, "logits", dt, {groups * beams, -1});
+  ck(lengths, "lengths", at::kInt, scores.sizes(), true);
+  ck(finished, "finished", at::kBool, scores.sizes(), true);
+  const int64_t vocab = logits.size(1);
+  int64_t tokens = 0;
+  if (sequences.has_value()) {
+    ck(*sequences, "sequences", at::kLong, {groups, beams, -1}, true);
+    tokens = sequences->size(2);
+  }
+  TORCH_CHECK(groups < INT32_MAX && beams < INT32_MAX && vocab < INT32_MAX && tokens < INT32_MAX, "beam_search_step: too many groups, beams, words or tokens");
+  BeamOut r = beam_outputs(scores, sequences);
+  if (groups == 0) return r;
+  const int64_t need = mmamd_beam_search_workspace((int)groups, (int)beams, (int)vocab);
+  const Tensor ws = workspace(need, "mmamd_beam_search_step", logits);
+  const bool seq = tokens > 0;
+  check_status(mmamd_beam_search_step(logits.data_ptr(), dt_code(dt), step(logits, 0), (const float*)ptr(scores), iptr(lengths), (const uint8_t*)ptr(finished),
+                                      seq ? (const int64_t*)ptr(*sequences) : nullptr, (int)tokens, eos, length_penalty, (int)groups, (int)beams, (int)vocab,
+                                      (float*)ptr(std::get<0>(r)), iptr(std::get<1>(r)), (uint8_t*)ptr(std::get<2>(r)), (int64_t*)ptr(std::get<3>(r)), iptr(std::get<4>(r)),
+                                      seq ? (int64_t*)ptr(std::get<5>(r)) : nullptr, ptr(ws), need, cur_stream(logits)),
+               "mmamd_beam_search_step");
+  return r;
+}
+BeamOut beam_search_step_meta(const Tensor&, const Tensor& scores, const Tensor&, const Tensor&, const OptTensor& sequences, int64_t, double) { return beam_outputs(scores, sequences); }
+
+}  // namespace
+
 TORCH_LIBRARY(mmamd, m) {
   m.def("abi_version() -> int", abi_version_impl);
   m.def("clear_packed() -> ()", clear_packed_impl);
@@ -497,6 +691,15 @@ TORCH_LIBRARY(mmamd, m) {
   m.def("rows_linear_f32(Tensor x, Tensor weight, Tensor? bias) -> Tensor");
   m.def("contrastive_fwd(Tensor a, Tensor b, Tensor a_all, Tensor b_all, Tensor logit_scale, int label_offset, Tensor? mask, "
         "float label_smoothing, int reduction) -> (Tensor, Tensor, Tensor)");
+  m.def("paged_attention(Tensor q, Tensor(a!) key_pages, Tensor(b!) value_pages, Tensor page_table, Tensor lengths, Tensor? k, Tensor? v, float? scale) -> Tensor");
+  m.def("paged_attention_into(Tensor q, Tensor(a!) key_pages, Tensor(b!) value_pages, Tensor page_table, Tensor lengths, Tensor? k, Tensor? v, float? scale, "
+        "Tensor(c!) out) -> ()");
+  m.def("paged_append(Tensor k, Tensor v, Tensor(a!) key_pages, Tensor(b!) value_pages, Tensor page_table, Tensor start, Tensor? counts) -> ()");
+  m.def("paged_fork(Tensor(a!) pages, Tensor page_table, Tensor lengths, Tensor refcounts, Tensor parents, Tensor? reserve_rows, int reserve) -> "
+        "(Tensor, Tensor, Tensor, Tensor)");
+  m.def("paged_compact(Tensor(a!) pages, Tensor page_table, Tensor refcounts) -> (Tensor, Tensor, Tensor)");
+  m.def("beam_search_step(Tensor logits, Tensor scores, Tensor lengths, Tensor finished, Tensor? sequences, int eos, float length_penalty) -> "
+        "(Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(mmamd, CUDA, m) {  // the "CUDA" dispatch key is the HIP device on ROCm builds of torch
@@ -518,6 +721,12 @@ TORCH_LIBRARY_IMPL(mmamd, CUDA, m) {  // the "CUDA" dispatch key is the HIP devi
   m.impl("coca_text_mask", coca_text_mask_impl);
   m.impl("rows_linear_f32", rows_linear_f32_impl);
   m.impl("contrastive_fwd", contrastive_fwd_impl);
+  m.impl("paged_attention", paged_attention_impl);
+  m.impl("paged_attention_into", paged_attention_into);
+  m.impl("paged_append", paged_append_impl);
+  m.impl("paged_fork", paged_fork_impl);
+  m.impl("paged_compact", paged_compact_impl);
+  m.impl("beam_search_step", beam_search_step_impl);
 }
 
 TORCH_LIBRARY_IMPL(mmamd, Meta, m) {
@@ -539,6 +748,12 @@ TORCH_LIBRARY_IMPL(mmamd, Meta, m) {
   m.impl("coca_text_mask", coca_text_mask_meta);
   m.impl("rows_linear_f32", rows_linear_f32_meta);
   m.impl("contrastive_fwd", contrastive_fwd_meta);
+  m.impl("paged_attention", paged_attention_meta);
+  m.impl("paged_attention_into", paged_attention_into_meta);
+  m.impl("paged_append", paged_append_meta);
+  m.impl("paged_fork", paged_fork_meta);
+  m.impl("paged_compact", paged_compact_meta);
+  m.impl("beam_search_step", beam_search_step_meta);
 }
 
 TORCH_LIBRARY_IMPL(mmamd, CompositeExplicitAutograd, m) { m.impl("allgather_packed", allgather_packed_impl); }

@@ -8,7 +8,6 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-from functools import lru_cache
 from typing import NamedTuple, Optional, Tuple, Union
 
 import torch
@@ -1435,61 +1434,28 @@ def target_rank(scores: torch.Tensor, target: Optional[torch.Tensor] = None) -> 
 
 
 # ---- decoding with a paged key-value cache --------------------------------------------------------------------------------------
+# A decoding step is short, so these go through the dispatcher ops (torch.ops.mmamd.*, csrc/torch_ops.cpp), which check and allocate in C++: one call took
+# 24-32 us of host time through ctypes with its checks in Python.  The C entry points underneath are the same ones (include/mmamd.h).
+
+_DECODING = None
 
 
-class _PagedCache(C.Structure):  # mmamd_paged_cache (include/mmamd.h)
-    _fields_ = [("key_pages", C.c_void_p), ("value_pages", C.c_void_p), ("page_table", C.c_void_p),
-                ("key_page_stride", C.c_int64), ("key_head_stride", C.c_int64), ("key_token_stride", C.c_int64),
-                ("value_page_stride", C.c_int64), ("value_head_stride", C.c_int64), ("value_token_stride", C.c_int64), ("table_row_stride", C.c_int64),
-                ("dtype", C.c_int32), ("pages", C.c_int32), ("page_size", C.c_int32), ("slots", C.c_int32), ("kv_heads", C.c_int32), ("dim", C.c_int32)]
+def _decoding():
+    global _DECODING
+    if _DECODING is None:
+        from . import _torch_ops
+
+        ns = _torch_ops.load()
+        _DECODING = {n: getattr(ns, n).default for n in ("paged_attention", "paged_attention_into", "paged_append", "paged_fork", "paged_compact", "beam_search_step")}
+    return _DECODING
 
 
-def _on(t: torch.Tensor, device: int, name: str, dtype: torch.dtype, shape, last: bool = True) -> None:
-    """t: a tensor of `dtype` and `shape` (None: any size) on the current device, its last axis contiguous where `last`."""
-    if not isinstance(t, torch.Tensor):
-        raise TypeError(f"{name} must be a tensor")
-    if not t.is_cuda:
-        raise MmamdError(f"{name} is on {t.device}: the MI355X path needs HIP device tensors (no CPU fallback)")
-    if t.get_device() != device:
-        raise MmamdError(f"{name} is on {t.device} but the current HIP device is cuda:{device}")
-    if t.dtype != dtype:
-        raise MmamdError(f"{name} must be {dtype}, got {t.dtype}")
-    got = t.shape
-    if len(got) != len(shape) or any(w is not None and g != w for g, w in zip(got, shape)):
-        raise MmamdError(f"{name} must have the shape {tuple('*' if w is None else w for w in shape)}, got {tuple(got)}")
-    if last and got[-1] > 1 and t.stride(-1) != 1 and t.numel() > 0:
-        raise MmamdError(f"{name} must be contiguous in its last axis")
-
-
-def _steps(t: torch.Tensor):
-    """Strides of all but the last axis; an axis of one entry is never stepped along, whatever its stride says."""
-    return [st if n > 1 else 0 for n, st in zip(t.shape[:-1], t.stride()[:-1])]
-
-
-def _no_grad(name: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise MmamdError(f"{name} has no gradient (decoding): call it under torch.no_grad()")
-
-
-def _size(need: int, what: str) -> int:
-    """The answer of a workspace function: a size, or an argument error."""
-    if need < 0:
-        check(int(need), what)
-    return int(need)
-
-
-def _paged_cache(key_pages: torch.Tensor, value_pages: torch.Tensor, page_table: torch.Tensor, rows: int, device: int) -> _PagedCache:
-    dt = key_pages.dtype if isinstance(key_pages, torch.Tensor) else None
-    if dt not in (torch.bfloat16, torch.float32):
-        raise MmamdError(f"key_pages must be a float32 or bfloat16 tensor, got {dt}")
-    _on(key_pages, device, "key_pages", dt, (None, None, None, None))
-    _on(value_pages, device, "value_pages", dt, key_pages.shape)
-    _on(page_table, device, "page_table", torch.int32, (rows, None))
-    n, heads, page, dim = key_pages.shape
-    if n == 0 or heads == 0 or page == 0 or page_table.shape[1] == 0:
-        raise MmamdError(f"pages {tuple(key_pages.shape)} and page_table {tuple(page_table.shape)} must not be empty")
-    return _PagedCache(key_pages.data_ptr(), value_pages.data_ptr(), page_table.data_ptr(), *_steps(key_pages), *_steps(value_pages), *_steps(page_table),
-                       F32 if dt == torch.float32 else BF16, n, page, page_table.shape[1], heads, dim)
+def _refused(name: str, e: Exception, tensors) -> MmamdError:
+    """The error of a dispatcher op in the form the other wrappers raise."""
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and not t.is_cuda and t.device.type != "meta":
+            return MmamdError(f"{name}: a tensor is on {t.device}: the MI355X path needs HIP device tensors (no CPU fallback)")
+    return MmamdError(str(e).split("\n")[0])
 
 
 def paged_attention(q: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor,
@@ -1500,38 +1466,15 @@ def paged_attention(q: torch.Tensor, key_pages: torch.Tensor, value_pages: torch
     q [rows, heads, dim]; key_pages / value_pages [pages, kv_heads, page_size, dim] (any strides, dim contiguous; dim 64, 96 or 128; bf16 or fp32, the same
     for all), heads a multiple of kv_heads; page_table int32 [rows, slots]; lengths int32 [rows] = tokens a row has in the cache.  With k, v [rows, kv_heads,
     dim] the new token is stored at position lengths[row] and seen; lengths are the caller's to advance.  Page numbers outside the pool hold no
-    tokens; a row that sees nothing gives zeros.  scale: 1 / sqrt(dim) unless given.  Two rows' new tokens must not share a place."""
-    device = torch.cuda.current_device() if torch.cuda.is_available() else -1
-    if not isinstance(q, torch.Tensor) or q.dim() != 3:
-        raise MmamdError("q must be a [rows, heads, dim] tensor")
-    rows, heads, dim = q.shape
-    cache = _paged_cache(key_pages, value_pages, page_table, rows, device)
-    dt = key_pages.dtype
-    _on(q, device, "q", dt, (rows, heads, cache.dim))
-    _on(lengths, device, "lengths", torch.int32, (rows,))
-    if (k is None) != (v is None):
-        raise MmamdError("k and v go together")
-    ks = vs = (0, 0)
-    if k is not None:
-        _on(k, device, "k", dt, (rows, cache.kv_heads, dim))
-        _on(v, device, "v", dt, (rows, cache.kv_heads, dim))
-        ks, vs = _steps(k), _steps(v)
-    _no_grad("paged_attention", q, k, v, key_pages, value_pages)
-    if out is None:
-        out = torch.empty((rows, heads, dim), dtype=dt, device=q.device)
-    else:
-        _on(out, device, "out", dt, (rows, heads, dim))
-        if not out.is_contiguous():
-            raise MmamdError("out must be contiguous")
-    if rows == 0:
+    tokens; a row that sees nothing gives zeros.  scale: 1 / sqrt(dim) unless given.  Two rows' new tokens must not share a place.  out: a contiguous
+    tensor for the result.  All tensors on one device, on whose current stream the work is put."""
+    try:
+        if out is None:
+            return _decoding()["paged_attention"](q, key_pages, value_pages, page_table, lengths, k, v, scale)
+        _decoding()["paged_attention_into"](q, key_pages, value_pages, page_table, lengths, k, v, scale, out)
         return out
-    lib = _lib.lib()
-    ref = C.byref(cache)
-    need = _size(lib.mmamd_paged_attention_workspace(ref, rows, heads), "mmamd_paged_attention")
-    ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    check(lib.mmamd_paged_attention(ref, lengths.data_ptr(), q.data_ptr(), *_steps(q), _ptr(k), *ks, _ptr(v), *vs, out.data_ptr(), rows, heads,
-                                    1.0 / math.sqrt(dim) if scale is None else float(scale), _ptr(ws), need, _stream()), "mmamd_paged_attention")
-    return out
+    except RuntimeError as e:
+        raise _refused("paged_attention", e, (q, key_pages, value_pages, page_table, lengths, k, v, out)) from e
 
 
 def paged_append(k: torch.Tensor, v: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, page_table: torch.Tensor, start: torch.Tensor,
@@ -1539,22 +1482,10 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, key_pages: torch.Tensor, valu
     """Stores prompts in the pages of a cache (mmamd_paged_append): token j < counts[row] (None: all of them) of k / v [rows, tokens, kv_heads, dim] goes to
     position start[row] + j; start, counts int32 [rows].  Tokens without a place (beyond the table, or on a page that is not mapped) are dropped, what lies
     behind counts[row] is not read.  Pages and table as in paged_attention."""
-    device = torch.cuda.current_device() if torch.cuda.is_available() else -1
-    if not isinstance(k, torch.Tensor) or k.dim() != 4:
-        raise MmamdError("k must be a [rows, tokens, kv_heads, dim] tensor")
-    rows, tokens, heads, dim = k.shape
-    cache = _paged_cache(key_pages, value_pages, page_table, rows, device)
-    dt = key_pages.dtype
-    _on(k, device, "k", dt, (rows, tokens, cache.kv_heads, cache.dim))
-    _on(v, device, "v", dt, k.shape)
-    _on(start, device, "start", torch.int32, (rows,))
-    if counts is not None:
-        _on(counts, device, "counts", torch.int32, (rows,))
-    _no_grad("paged_append", k, v, key_pages, value_pages)
-    if k.numel() == 0:
-        return
-    check(_lib.lib().mmamd_paged_append(C.byref(cache), k.data_ptr(), *_steps(k), v.data_ptr(), *_steps(v), start.data_ptr(), _ptr(counts), rows, tokens,
-                                        _stream()), "mmamd_paged_append")
+    try:
+        _decoding()["paged_append"](k, v, key_pages, value_pages, page_table, start, counts)
+    except RuntimeError as e:
+        raise _refused("paged_append", e, (k, v, key_pages, value_pages, page_table, start, counts)) from e
 
 
 class PagedState(NamedTuple):
@@ -1572,20 +1503,6 @@ class CompactedPages(NamedTuple):
     live: torch.Tensor
 
 
-def _pool(pages: torch.Tensor, refcounts: torch.Tensor, device: int) -> None:
-    if not isinstance(pages, torch.Tensor) or pages.dtype not in (torch.bfloat16, torch.float32) or pages.dim() < 3:
-        raise MmamdError("pages must be a float32 or bfloat16 tensor [pages, ..., page_size, dim]")
-    _on(pages, device, "pages", pages.dtype, (None,) * pages.dim())
-    if not pages.is_contiguous() or pages.numel() == 0:
-        raise MmamdError(f"pages must be contiguous and not empty, got {tuple(pages.shape)}")
-    _on(refcounts, device, "refcounts", torch.int32, (pages.shape[0],))
-
-
-@lru_cache(maxsize=256)
-def _fork_workspace(old_rows: int, rows: int, slots: int, pages: int) -> int:
-    return _size(_lib.lib().mmamd_paged_fork_workspace(old_rows, rows, slots, pages), "mmamd_paged_fork")
-
-
 def paged_fork(pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Tensor, refcounts: torch.Tensor, parents: torch.Tensor,
                reserve: Union[int, torch.Tensor] = 0) -> PagedState:
     """New rows from old ones (mmamd_paged_fork): row r continues the old row parents[r] (int32; -1: an empty row), sharing its full pages; of a partial last
@@ -1595,61 +1512,20 @@ def paged_fork(pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Ten
     pages: the whole pool [pages, ..., page_size, dim], contiguous (every layer's keys and values of a page together, so that one call serves them all);
     page_table int32 [old rows, slots], lengths int32 [old rows], refcounts int32 [pages] = table entries a page stands in (not positive: free).  Fresh
     pages are the lowest free ones, in the order of the new entries.  Only the copied pages are written, the old state stays as it was."""
-    device = torch.cuda.current_device() if torch.cuda.is_available() else -1
-    _pool(pages, refcounts, device)
-    _on(page_table, device, "page_table", torch.int32, (None, None))
-    old_rows, slots = page_table.shape
-    _on(lengths, device, "lengths", torch.int32, (old_rows,))
-    _on(parents, device, "parents", torch.int32, (None,))
-    rows, n = parents.shape[0], pages.shape[0]
-    if slots == 0:
-        raise MmamdError("page_table must have at least one slot")
     per_row = isinstance(reserve, torch.Tensor)
-    if per_row:
-        _on(reserve, device, "reserve", torch.int32, (rows,))
-    elif not 0 <= int(reserve) < 1 << 31:
-        raise MmamdError(f"reserve must be a number of tokens, got {reserve}")
-    page, dim = pages.shape[-2:]
-    lib = _lib.lib()
-    need = _fork_workspace(old_rows, rows, slots, n)
-    dev = pages.device
-    table = torch.empty((rows, slots), dtype=torch.int32, device=dev)
-    lens = torch.empty((rows,), dtype=torch.int32, device=dev)
-    counts = torch.empty((n,), dtype=torch.int32, device=dev)
-    short = torch.empty((1,), dtype=torch.int32, device=dev)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    check(lib.mmamd_paged_fork(pages.data_ptr(), n, pages.numel() // (n * page * dim), page, dim * pages.element_size(), page_table.data_ptr(), *_steps(page_table),
-                               lengths.data_ptr(), refcounts.data_ptr(), old_rows, slots, parents.data_ptr(), rows, reserve.data_ptr() if per_row else None,
-                               0 if per_row else int(reserve), table.data_ptr(), lens.data_ptr(), counts.data_ptr(), short.data_ptr(), ws.data_ptr(), need,
-                               _stream()), "mmamd_paged_fork")
-    return PagedState(table, lens, counts, short)
-
-
-@lru_cache(maxsize=256)
-def _compact_workspace(pages: int) -> int:
-    return _size(_lib.lib().mmamd_paged_compact_workspace(pages), "mmamd_paged_compact")
+    try:
+        return PagedState(*_decoding()["paged_fork"](pages, page_table, lengths, refcounts, parents, reserve if per_row else None, 0 if per_row else reserve))
+    except RuntimeError as e:
+        raise _refused("paged_fork", e, (pages, page_table, lengths, refcounts, parents, reserve)) from e
 
 
 def paged_compact(pages: torch.Tensor, page_table: torch.Tensor, refcounts: torch.Tensor) -> CompactedPages:
     """Moves the live pages with the highest numbers into the lowest free places (mmamd_paged_compact): afterwards pages 0 .. live - 1 are the live ones, and
     the rest of the pool can be given back.  Arguments as in paged_fork; table entries whose page is not live become -1."""
-    device = torch.cuda.current_device() if torch.cuda.is_available() else -1
-    _pool(pages, refcounts, device)
-    _on(page_table, device, "page_table", torch.int32, (None, None))
-    rows, slots = page_table.shape
-    n = pages.shape[0]
-    if slots == 0:
-        raise MmamdError("page_table must have at least one slot")
-    need = _compact_workspace(n)
-    dev = pages.device
-    table = torch.empty((rows, slots), dtype=torch.int32, device=dev)
-    counts = torch.empty((n,), dtype=torch.int32, device=dev)
-    live = torch.empty((1,), dtype=torch.int32, device=dev)
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    check(_lib.lib().mmamd_paged_compact(pages.data_ptr(), n, pages.numel() // n * pages.element_size(), page_table.data_ptr(), *_steps(page_table), rows, slots,
-                                         refcounts.data_ptr(), table.data_ptr(), counts.data_ptr(), live.data_ptr(), ws.data_ptr(), need, _stream()),
-          "mmamd_paged_compact")
-    return CompactedPages(table, counts, live)
+    try:
+        return CompactedPages(*_decoding()["paged_compact"](pages, page_table, refcounts))
+    except RuntimeError as e:
+        raise _refused("paged_compact", e, (pages, page_table, refcounts)) from e
 
 
 class BeamStep(NamedTuple):
@@ -1663,11 +1539,6 @@ class BeamStep(NamedTuple):
     sequences: Optional[torch.Tensor]
 
 
-@lru_cache(maxsize=256)
-def _beam_workspace(groups: int, beams: int, vocab: int) -> int:
-    return _size(_lib.lib().mmamd_beam_search_workspace(groups, beams, vocab), "mmamd_beam_search_step")
-
-
 def beam_search_step(logits: torch.Tensor, scores: torch.Tensor, lengths: torch.Tensor, finished: torch.Tensor, sequences: Optional[torch.Tensor], eos: int,
                      length_penalty: float = 0.0) -> BeamStep:
     """One step of a beam search (mmamd_beam_search_step): of all continuations of a group's beams the best, and the reordered state.
@@ -1676,33 +1547,8 @@ def beam_search_step(logits: torch.Tensor, scores: torch.Tensor, lengths: torch.
     tokens] or None.  A beam that goes on offers scores + log_softmax(logits), a finished one only itself (as token `eos`).  The best by
     total / max(length, 1) ** length_penalty win, ties go to the lowest beam * vocab + token; ranked in 64 bits.  A search begins with scores 0 for the
     first beam of a group and -inf for the others.  parents is what paged_fork takes (flattened)."""
-    device = torch.cuda.current_device() if torch.cuda.is_available() else -1
-    if not isinstance(logits, torch.Tensor) or logits.dtype not in (torch.float32, torch.bfloat16):
-        raise MmamdError("logits must be a float32 or bfloat16 tensor [groups * beams, vocab]")
-    _on(scores, device, "scores", torch.float32, (None, None))
-    groups, beams = shape = tuple(scores.shape)
-    _on(logits, device, "logits", logits.dtype, (groups * beams, None))
-    _on(lengths, device, "lengths", torch.int32, shape)
-    _on(finished, device, "finished", torch.bool, shape)
-    vocab = logits.shape[1]
-    tokens = 0
-    if sequences is not None:
-        _on(sequences, device, "sequences", torch.int64, (groups, beams, None))
-        tokens = sequences.shape[2]
-    for t, name in ((scores, "scores"), (lengths, "lengths"), (finished, "finished"), (sequences, "sequences")):
-        if t is not None and not t.is_contiguous():
-            raise MmamdError(f"{name} must be contiguous")
-    _no_grad("beam_search_step", logits, scores)
-    lib = _lib.lib()
-    need = _beam_workspace(groups, beams, vocab)
-    dev = logits.device
-    r = BeamStep(torch.empty(shape, dtype=torch.float32, device=dev), torch.empty(shape, dtype=torch.int32, device=dev), torch.empty(shape, dtype=torch.bool, device=dev),
-                 torch.empty(shape, dtype=torch.int64, device=dev), torch.empty(shape, dtype=torch.int32, device=dev),
-                 None if sequences is None else torch.empty_like(sequences))
-    if groups == 0:
-        return r
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    check(lib.mmamd_beam_search_step(logits.data_ptr(), _dt(logits), *_steps(logits), scores.data_ptr(), lengths.data_ptr(), finished.data_ptr(), _ptr(sequences), tokens,
-                                     int(eos), float(length_penalty), groups, beams, vocab, r.scores.data_ptr(), r.lengths.data_ptr(), r.finished.data_ptr(),
-                                     r.tokens.data_ptr(), r.parents.data_ptr(), _ptr(r.sequences), ws.data_ptr(), need, _stream()), "mmamd_beam_search_step")
-    return r
+    try:
+        r = _decoding()["beam_search_step"](logits, scores, lengths, finished, sequences, eos, length_penalty)
+    except RuntimeError as e:
+        raise _refused("beam_search_step", e, (logits, scores, lengths, finished, sequences)) from e
+    return BeamStep(*r) if sequences is not None else BeamStep(*r[:5], None)

@@ -15,8 +15,9 @@ def place(table, row, t, page, pages):
     return (p, t % page) if 0 <= p < pages else None
 
 
-def paged_attention(q, key_pages, value_pages, table, lengths, k=None, v=None, scale=None):
-    """(out [rows, heads, dim] float64, key_pages, value_pages after the call, err): err bounds what 32-bit arithmetic may lose, see `fp32_loss`."""
+def paged_attention(q, key_pages, value_pages, table, lengths, k=None, v=None, scale=None, weight_loss=0.0):
+    """(out [rows, heads, dim] float64, key_pages, value_pages after the call, err): err bounds what 32-bit arithmetic may lose, see `fp32_loss`,
+    and a loss of `weight_loss` of every weight."""
     kp, vp = key_pages.copy(), value_pages.copy()
     rows, heads, dim = q.shape
     pages, kv_heads, page, _ = kp.shape
@@ -43,7 +44,7 @@ def paged_attention(q, key_pages, value_pages, table, lengths, k=None, v=None, s
             w = np.exp(s - s.max())
             w /= w.sum()
             out[r, h] = w @ vv
-            err[r, h] = fp32_loss(scale * (np.abs(kk) @ np.abs(qq)).max(), dim, len(places)) * (w @ np.abs(vv))
+            err[r, h] = (fp32_loss(scale * (np.abs(kk) @ np.abs(qq)).max(), dim, len(places)) + weight_loss) * (w @ np.abs(vv))
     return out, kp, vp, err
 
 

@@ -21,9 +21,14 @@ def L():
     return _lib.lib()
 
 
-def cache(**kw):
-    from multimodal_amd.ops import _PagedCache
+class _PagedCache(C.Structure):  # mmamd_paged_cache (include/mmamd.h)
+    _fields_ = [("key_pages", C.c_void_p), ("value_pages", C.c_void_p), ("page_table", C.c_void_p),
+                ("key_page_stride", C.c_int64), ("key_head_stride", C.c_int64), ("key_token_stride", C.c_int64),
+                ("value_page_stride", C.c_int64), ("value_head_stride", C.c_int64), ("value_token_stride", C.c_int64), ("table_row_stride", C.c_int64),
+                ("dtype", C.c_int32), ("pages", C.c_int32), ("page_size", C.c_int32), ("slots", C.c_int32), ("kv_heads", C.c_int32), ("dim", C.c_int32)]
 
+
+def cache(**kw):
     d = dict(key_pages=4096, value_pages=8192, page_table=64, key_page_stride=2048, key_head_stride=1024, key_token_stride=64, value_page_stride=2048,
              value_head_stride=1024, value_token_stride=64, table_row_stride=4, dtype=1, pages=8, page_size=16, slots=4, kv_heads=2, dim=64)
     d.update(kw)
@@ -88,22 +93,30 @@ def test_wrappers_refuse_host_tensors_and_wrong_types():
     from multimodal_amd import ops
 
     q, pages, table, n = torch.zeros(1, 2, 64), torch.zeros(4, 2, 16, 64), torch.zeros(1, 2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32)
-    with pytest.raises(ops.MmamdError, match="no CPU fallback"):
-        ops.paged_attention(q, pages, pages, table, n)
-    with pytest.raises(ops.MmamdError, match="float32 or bfloat16"):
-        ops.paged_attention(q, pages.half(), pages.half(), table, n)
-    with pytest.raises(ops.MmamdError, match="tensor"):
-        ops.paged_attention(q[0], pages, pages, table, n)
-    with pytest.raises(ops.MmamdError, match="no CPU fallback"):
-        ops.paged_append(q[None], q[None], pages, pages, table, n)
-    with pytest.raises(ops.MmamdError, match="no CPU fallback"):
-        ops.paged_fork(pages, table, n, n, n)
-    with pytest.raises(ops.MmamdError, match="no CPU fallback"):
-        ops.paged_compact(pages, table, n)
-    with pytest.raises(ops.MmamdError, match="no CPU fallback"):
-        ops.beam_search_step(torch.zeros(2, 5), torch.zeros(1, 2), table, table.bool(), None, 0)
-    with pytest.raises(ops.MmamdError, match="float32 or bfloat16"):
-        ops.beam_search_step(torch.zeros(2, 5).double(), torch.zeros(1, 2), table, table.bool(), None, 0)
+    calls = [lambda: ops.paged_attention(q, pages, pages, table, n), lambda: ops.paged_attention(q, pages, pages, table, n, out=q),
+             lambda: ops.paged_append(q[None], q[None], pages, pages, table, n), lambda: ops.paged_fork(pages, table, n, n, n),
+             lambda: ops.paged_compact(pages, table, n), lambda: ops.beam_search_step(torch.zeros(2, 5), torch.zeros(1, 2), table, table.bool(), None, 0)]
+    for call in calls:
+        with pytest.raises(ops.MmamdError, match="no CPU fallback"):
+            call()
+    with pytest.raises(ops.MmamdError):
+        ops.paged_attention(1.0, 2, 3, table, n)
+
+
+def test_meta_kernels_infer_shapes():
+    from multimodal_amd import _torch_ops
+
+    ns = _torch_ops.load()
+    m = lambda *s, dtype=torch.float32: torch.empty(*s, dtype=dtype, device="meta")  # noqa: E731
+    i = torch.int32
+    out = ns.paged_attention(m(3, 4, 64), m(9, 2, 16, 64), m(9, 2, 16, 64), m(3, 5, dtype=i), m(3, dtype=i), None, None, None)
+    assert out.shape == (3, 4, 64)
+    table, lengths, refs, short = ns.paged_fork(m(9, 2, 16, 64), m(3, 5, dtype=i), m(3, dtype=i), m(9, dtype=i), m(7, dtype=i), None, 1)
+    assert table.shape == (7, 5) and lengths.shape == (7,) and refs.shape == (9,) and short.shape == (1,) and table.dtype == i
+    assert [tuple(t.shape) for t in ns.paged_compact(m(9, 2, 16, 64), m(3, 5, dtype=i), m(9, dtype=i))] == [(3, 5), (9,), (1,)]
+    r = ns.beam_search_step(m(6, 50), m(2, 3), m(2, 3, dtype=i), m(2, 3, dtype=torch.bool), m(2, 3, 8, dtype=torch.int64), 1, 0.0)
+    assert [t.dtype for t in r] == [torch.float32, i, torch.bool, torch.int64, i, torch.int64] and r[5].shape == (2, 3, 8)
+    assert "Tensor(a!) key_pages" in str(ns.paged_attention.default._schema)
 
 
 def test_page_division(tmp_path):
