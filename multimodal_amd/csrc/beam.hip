@@ -27,18 +27,23 @@ struct BeamParams {
   int64_t *out_tokens, *out_sequences;
   float* unit_max;      // workspace, per row and unit
   double* unit_sum;
-  uint2* unit_top;      // per row, unit and place: (order key, index); key 0 = none
+  uint2* unit_top;      // per row, unit and place: (logit, index), best first; index -1 = none
   int groups, beams, vocab, units, tokens;
   double penalty;
 };
 
-// floats in the order of unsigned integers; NaN counts as -inf here (a row that holds one is dead by its sum)
-__device__ __forceinline__ uint32_t order_key(float x) {
-  const uint32_t u = __float_as_uint(x);
-  const uint32_t k = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-  return x == x ? k : 0x007fffffu;  // the key of -inf
+// a wave's maximum, in every lane, by data-parallel moves (a shuffle goes through LDS); NaN counts as nothing
+__device__ __forceinline__ float dpp_max(float v) {
+#define MMAMD_DPP_MAX(ctrl, rows) v = fmaxf(v, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), ctrl, rows, 0xf, false)))
+  MMAMD_DPP_MAX(0x111, 0xf);  // row_shr:1, 2, 4, 8: lane 15 of each row of 16 has the row's
+  MMAMD_DPP_MAX(0x112, 0xf);
+  MMAMD_DPP_MAX(0x114, 0xf);
+  MMAMD_DPP_MAX(0x118, 0xf);
+  MMAMD_DPP_MAX(0x142, 0xa);  // row_bcast:15 and :31: lane 63 has all
+  MMAMD_DPP_MAX(0x143, 0xc);
+#undef MMAMD_DPP_MAX
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
-__device__ __forceinline__ float key_value(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
 
 template <typename T>
 __device__ __forceinline__ void beam_load4(const T* p, bool vec, int left, float (&f)[4]) {
@@ -52,91 +57,142 @@ __device__ __forceinline__ void beam_load4(const T* p, bool vec, int left, float
   }
 }
 
-// grid: ceil(units / 4) x rows, one unit a wave
+// grid: ceil(units / 4) x rows, one unit a wave.  Of the lanes' maxima the `beams`-th highest is a bound that the unit's `beams` best do not fall below:
+// what lies above it (31 values for each of fewer than `beams` lanes, at most, a handful as a rule) and the first of its equals are gathered in LDS,
+// where each counts how many are better.  (Taking the best `beams` times over all 32 values of a lane was bound by its compares and shuffles: 39 us for
+// 512 rows of 49408, 12 us for 5.)
 template <typename T>
 __global__ __launch_bounds__(256) void beam_scan_kernel(const BeamParams p) {
-  const int row = blockIdx.y, unit = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  extern __shared__ uint2 lists[];
+  const int row = blockIdx.y, unit = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63, K = p.beams;
   if (unit >= p.units || p.finished[row] || !(p.scores[row] > -INFINITY)) return;  // nobody reads the units of such a row
+  uint2* list = lists + (threadIdx.x >> 6) * 32 * K;
   const T* x = reinterpret_cast<const T*>(p.logits) + row * p.ld;
   const bool vec = (reinterpret_cast<uintptr_t>(x) & (4 * sizeof(T) - 1)) == 0;
   const int base = unit * kBeamUnit + lane * 4;
   float f[8][4];
 #pragma unroll
   for (int i = 0; i < 8; ++i) beam_load4<T>(x + base + i * 256, vec, p.vocab - (base + i * 256), f[i]);
-  float top = -INFINITY;
-  uint32_t key[8][4];
+  float mine = -INFINITY;
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      top = fmaxf(top, f[i][j]);
-      key[i][j] = base + i * 256 + j < p.vocab ? order_key(f[i][j]) : 0u;
-    }
-  top = wave_max(top);
-  // 32 terms a lane in 32 bits, the lanes in 64.  With no maximum (all -inf) there is no sum either; a NaN or +inf makes it NaN.
+    for (int j = 0; j < 4; ++j) mine = fmaxf(mine, f[i][j]);
+  const float top = dpp_max(mine);
+  // 32 terms a lane in 32 bits, the lanes in 64; the difference first, so that the terms that count are the exact ones.  With no maximum (all -inf) there
+  // is no sum; a NaN or +inf makes it NaN.
   float part = 0.f;
-  bool nan = false;
 #pragma unroll
   for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (base + i * 256 + j < p.vocab) nan |= !(f[i][j] < INFINITY);
-      part += top > -INFINITY ? expf(f[i][j] - top) : 0.f;
-    }
-  double sum = (double)part;
+    for (int j = 0; j < 4; ++j) part += __builtin_amdgcn_exp2f((f[i][j] - top) * 1.4426950408889634f);
+  double sum = top > -INFINITY ? (double)part : 0.0;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-  if (__any(nan)) sum = NAN;
+  if (__any(!(part == part)) && top > -INFINITY) sum = NAN;
   const int64_t at = (int64_t)row * p.units + unit;
-  if (lane == 0) { p.unit_max[at] = top; p.unit_sum[at] = sum; }
-  for (int k = 0; k < p.beams; ++k) {
-    uint32_t best = 0;
-    int where = 0;
+  if (top == -INFINITY) {  // nothing but -inf, or NaN and -inf: told apart here
+    bool nan = false;
 #pragma unroll
     for (int i = 0; i < 8; ++i)
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (key[i][j] > best) { best = key[i][j]; where = i * 4 + j; }
-    uint32_t all = best;
+      for (int j = 0; j < 4; ++j) nan |= !(f[i][j] == f[i][j]);
+    if (__any(nan)) sum = NAN;
+  }
+  if (lane == 0) { p.unit_max[at] = top; p.unit_sum[at] = sum; }
+
+  float left = mine, bound = top;
+  for (int k = 0; k < K && bound > -INFINITY; ++k) {
+    bound = dpp_max(left);
+    const unsigned long long who = __ballot(left == bound);
+    if (lane == __ffsll(who) - 1) left = -INFINITY;
+  }
+  int n = 0;  // gathered, the same in every lane
+  const unsigned long long below = (1ull << lane) - 1;
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) { const uint32_t y = __shfl_xor(all, o); all = y > all ? y : all; }
-    const int idx = base + (where >> 2) * 256 + (where & 3);
-    int low = best == all && all != 0 ? idx : 0x7fffffff;
+  for (int i = 0; i < 8; ++i)
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) { const int y = __shfl_xor(low, o); low = y < low ? y : low; }
-    if (lane == 0) p.unit_top[at * p.beams + k] = make_uint2(all, (uint32_t)low);
-    if (all != 0 && low == idx) {
+    for (int j = 0; j < 4; ++j) {
+      const unsigned long long who = __ballot(f[i][j] > bound);
+      if (who != 0) {
+        if (f[i][j] > bound) list[n + __popcll(who & below)] = make_uint2(__float_as_uint(f[i][j]), (uint32_t)(base + i * 256 + j));
+        n += __popcll(who);
+      }
+    }
+  if (bound > -INFINITY) {
+    const int above = n;
+    int equal = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 8; ++i) {
+      int before = 0, all = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const unsigned long long who = __ballot(f[i][j] == bound);
+        before += __popcll(who & below);
+        all += __popcll(who);
+      }
+      if (all != 0 && above + equal < K) {
+        int rank = equal + before;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          if (where == i * 4 + j) key[i][j] = 0;
+          if (f[i][j] == bound) {
+            if (above + rank < K) list[above + rank] = make_uint2(__float_as_uint(bound), (uint32_t)(base + i * 256 + j));
+            ++rank;
+          }
+      }
+      equal += all;
     }
+    n = above + equal < K ? above + equal : (above > K ? above : K);
   }
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's list is in LDS
+  uint2* out = p.unit_top + at * K;
+  for (int e = lane; e < n; e += 64) {
+    const uint2 me = list[e];
+    const float v = __uint_as_float(me.x);
+    int better = 0;
+    for (int d = 0; d < n; ++d) {
+      const uint2 y = list[d];
+      const float w = __uint_as_float(y.x);
+      better += w > v || (w == v && y.y < me.y);
+    }
+    if (better < K) out[better] = me;
+  }
+  if (lane >= n && lane < K) out[lane] = make_uint2(0xff800000u, 0xffffffffu);  // none
 }
-
-// is (key, index) of one candidate of a beam behind another's: lower, or as high and further back
-__device__ __forceinline__ bool behind(uint32_t k, uint32_t i, uint32_t k0, uint32_t i0) { return k < k0 || (k == k0 && i > i0); }
 
 // One workgroup per group.  A wave per beam joins the sums and merges the units' lists into the beam's `beams` best; the continuations of all beams then
 // count how many are better than they, which is their place.
-__global__ __launch_bounds__(256) void beam_join_kernel(const BeamParams p) {
+__global__ __launch_bounds__(512) void beam_join_kernel(const BeamParams p) {
   __shared__ double rank[kBeamMost * kBeamMost];
   __shared__ float total[kBeamMost * kBeamMost];
   __shared__ uint32_t token[kBeamMost * kBeamMost];
   __shared__ int place[kBeamMost];
   const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, K = p.beams;
-  for (int b = wave; b < K; b += 4) {
+  for (int b = wave; b < K; b += blockDim.x >> 6) {
     const int row = g * K + b;
     const bool fin = p.finished[row] != 0;
     const double score = (double)p.scores[row];
+    const int count = p.units * K;
+    const uint2* list = p.unit_top + (int64_t)row * count;
+    const float* um = p.unit_max + (int64_t)row * p.units;
+    const double* us = p.unit_sum + (int64_t)row * p.units;
+    const bool on = !fin && score > -INFINITY;
+    // up to four candidates a lane are kept in registers, more are read again for every place
+    const bool few = count <= 256;
+    float cv[4];
+    uint32_t ci[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int c = lane + j * 64;
+      const uint2 e = on && few && c < count ? list[c] : make_uint2(0xff800000u, 0xffffffffu);
+      cv[j] = __uint_as_float(e.x);
+      ci[j] = e.y;
+    }
     double lse = NAN;
-    if (!fin && score > -INFINITY) {
-      const float* um = p.unit_max + (int64_t)row * p.units;
-      const double* us = p.unit_sum + (int64_t)row * p.units;
+    if (on) {
       float top = -INFINITY;
       for (int u = lane; u < p.units; u += 64) top = fmaxf(top, um[u]);
-      top = wave_max(top);
+      top = dpp_max(top);
       double sum = 0.0;
       for (int u = lane; u < p.units; u += 64) sum += um[u] > -INFINITY ? us[u] * exp((double)um[u] - (double)top) : us[u];
 #pragma unroll
@@ -144,29 +200,57 @@ __global__ __launch_bounds__(256) void beam_join_kernel(const BeamParams p) {
       lse = (double)top + log(sum);
     }
     const int len = p.lengths[row] + (fin ? 0 : 1);
-    const double div = pow((double)(len > 1 ? len : 1), p.penalty);
+    const double base = (double)(len > 1 ? len : 1);
+    const double div = p.penalty == 0.0 ? 1.0 : p.penalty == 1.0 ? base : pow(base, p.penalty);
     if (lse > -INFINITY && lse < INFINITY) {
-      const uint2* list = p.unit_top + (int64_t)row * p.units * K;
-      uint32_t k0 = 0xffffffffu, i0 = 0;
-      for (int k = 0; k < K; ++k) {
-        uint32_t bk = 0, bi = 0xffffffffu;
-        for (int c = lane; c < p.units * K; c += 64) {
-          const uint2 e = list[c];
-          if (e.x != 0 && behind(e.x, e.y, k0, i0) && (e.x > bk || (e.x == bk && e.y < bi))) { bk = e.x; bi = e.y; }
-        }
+      float v0 = INFINITY;
+      uint32_t i0 = 0;
+      int found = 0;
+      for (; found < K; ++found) {
+        float bv = -INFINITY;
+        uint32_t bi = 0xffffffffu;
+        if (few) {
 #pragma unroll
-        for (int o = 32; o > 0; o >>= 1) {
-          const uint32_t yk = __shfl_xor(bk, o), yi = __shfl_xor(bi, o);
-          if (yk > bk || (yk == bk && yi < bi)) { bk = yk; bi = yi; }
+          for (int j = 0; j < 4; ++j)
+            if (cv[j] > bv || (cv[j] == bv && ci[j] < bi)) { bv = cv[j]; bi = ci[j]; }
+        } else {
+          for (int c = lane; c < count; c += 64) {
+            const uint2 e = list[c];
+            const float v = __uint_as_float(e.x);
+            if ((v < v0 || (v == v0 && e.y > i0)) && (v > bv || (v == bv && e.y < bi))) { bv = v; bi = e.y; }
+          }
         }
+        const float best = dpp_max(bv);
+        if (!(best > -INFINITY)) break;
+        uint32_t low = bv == best ? bi : 0xffffffffu;
+        const unsigned long long who = __ballot(bv == best);
+        if ((who & (who - 1)) == 0) {
+          low = (uint32_t)__builtin_amdgcn_readlane((int)bi, __ffsll(who) - 1);
+        } else {
+#pragma unroll
+          for (int o = 32; o > 0; o >>= 1) { const uint32_t y = __shfl_xor(low, o); low = y < low ? y : low; }
+        }
+        v0 = best;
+        i0 = low;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (ci[j] == low) { cv[j] = -INFINITY; ci[j] = 0xffffffffu; }
         if (lane == 0) {
-          const float logit = key_value(bk);
-          const double t = bk != 0 && logit > -INFINITY ? score + ((double)logit - lse) : -INFINITY;
-          rank[b * K + k] = t / div;
-          total[b * K + k] = (float)t;
-          token[b * K + k] = bk != 0 ? bi : 0xffffffffu;  // (a vocabulary smaller than the beams)
+          const double t = score + ((double)best - lse);
+          rank[b * K + found] = t / div;
+          total[b * K + found] = (float)t;
+          token[b * K + found] = low;
         }
-        k0 = bk; i0 = bi;
+      }
+      if (found < K && lane == 0) {  // all finite ones are listed: the first words that are not, at -inf
+        uint32_t t = 0;
+        for (int k = found; k < K; ++k, ++t) {
+          for (int d = 0; d < found; ++d)
+            if (token[b * K + d] == t) { ++t; d = -1; }
+          rank[b * K + k] = -INFINITY;
+          total[b * K + k] = -INFINITY;
+          token[b * K + k] = t < (uint32_t)p.vocab ? t : 0xffffffffu;
+        }
       }
     } else if (lane < K) {
       // a finished beam goes on as it is; every other continuation of it, and all of a dead beam, tie at -inf: the first ones of them
@@ -175,33 +259,33 @@ __global__ __launch_bounds__(256) void beam_join_kernel(const BeamParams p) {
       const int t = !alive ? lane : lane == 0 ? eos : (lane - 1 < eos ? lane - 1 : lane);
       const double own = alive && lane == 0 ? score : -INFINITY;
       rank[b * K + lane] = own / div;
-      token[b * K + lane] = t < p.vocab ? (uint32_t)t : 0xffffffffu;
       total[b * K + lane] = (float)own;
+      token[b * K + lane] = t < p.vocab ? (uint32_t)t : 0xffffffffu;
     }
   }
   __syncthreads();
-  for (int c = tid; c < K * K; c += 256) {
-    if (token[c] == 0xffffffffu) continue;
+  for (int c = tid; c < K * K; c += blockDim.x) {
+    if (token[c] == 0xffffffffu) continue;  // (a vocabulary smaller than the beams)
     const double r = rank[c];
     const int64_t flat = (int64_t)(c / K) * p.vocab + token[c];
-    int better = 0;
-    for (int d = 0; d < K * K; ++d)
-      better += token[d] != 0xffffffffu && (rank[d] > r || (rank[d] == r && (int64_t)(d / K) * p.vocab + token[d] < flat));
+    int better = 0, d = 0;
+    for (int b = 0; b < K; ++b)
+      for (int k = 0; k < K; ++k, ++d)
+        better += token[d] != 0xffffffffu && (rank[d] > r || (rank[d] == r && (int64_t)b * p.vocab + token[d] < flat));
     if (better < K) place[better] = c;
   }
   __syncthreads();
-  for (int k = tid; k < K; k += 256) {
-    const int c = place[k], b = c / K, row = g * K + b, to = g * K + k;
+  for (int k = tid; k < K; k += blockDim.x) {
+    const int c = place[k], row = g * K + c / K, to = g * K + k;
     const bool fin = p.finished[row] != 0;
-    const int len = p.lengths[row] + (fin ? 0 : 1);
     p.out_scores[to] = total[c];
-    p.out_lengths[to] = len;
+    p.out_lengths[to] = p.lengths[row] + (fin ? 0 : 1);
     p.out_finished[to] = fin || token[c] == (uint32_t)p.eos;
     p.out_tokens[to] = token[c];
     p.out_parents[to] = row;
   }
   if (p.out_sequences == nullptr) return;
-  for (int64_t i = tid; i < (int64_t)K * p.tokens; i += 256) {
+  for (int64_t i = tid; i < (int64_t)K * p.tokens; i += blockDim.x) {
     const int k = (int)(i / p.tokens), t = (int)(i - (int64_t)k * p.tokens);
     const int c = place[k], row = g * K + c / K;
     const bool put = p.finished[row] == 0 && t == p.lengths[row];
@@ -249,9 +333,10 @@ extern "C" int mmamd_beam_search_step(const void* logits, int dtype, int64_t ld,
   p.unit_max = reinterpret_cast<float*>(p.unit_sum + n);
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid((p.units + 3) / 4, groups * beams);
-  if (dtype == MMAMD_F32) beam_scan_kernel<float><<<grid, 256, 0, st>>>(p);
-  else beam_scan_kernel<bf16><<<grid, 256, 0, st>>>(p);
+  const int lds = 4 * 32 * beams * 8;  // at most 32 values of `beams` lanes in the list of each wave: 32 KiB
+  if (dtype == MMAMD_F32) beam_scan_kernel<float><<<grid, 256, lds, st>>>(p);
+  else beam_scan_kernel<bf16><<<grid, 256, lds, st>>>(p);
   if (int rc = launch_status("beam_search_step scan")) return rc;
-  beam_join_kernel<<<groups, 256, 0, st>>>(p);
+  beam_join_kernel<<<groups, 64 * (beams < 8 ? beams : 8), 0, st>>>(p);
   return launch_status("beam_search_step");
 }

@@ -10,7 +10,8 @@ struct ForkParams {
   char* pool;
   const int32_t *table, *lengths, *refs, *parents, *reserve_rows;
   int32_t *new_table, *new_lengths, *new_refs, *shortage;
-  int32_t *first, *children, *base, *src, *fresh, *found;  // workspace: two per old row, two per new row, the fresh pages and how many there are
+  int32_t *first, *children, *base, *src, *fresh, *found;  // workspace: two per old row, two per new row, the fresh pages, how many there are and how many copies
+  int4* copies;                                            // from page, to page, tokens
   int64_t table_row;
   int old_rows, rows, pages, slots, reserve, fresh_max;
   int64_t page_bytes, block_bytes, row_bytes;
@@ -122,56 +123,82 @@ __global__ __launch_bounds__(1024) void paged_fork_plan_kernel(const ForkParams 
     found += total;
   }
   if (found > needed) found = needed;
-  if (tid == 0) { p.found[0] = found; p.shortage[0] = needed - found; }
+  __threadfence_block();
+  int copies = 0;
+  for (int r0 = 0; r0 < p.rows; r0 += 1024) {
+    const int r = r0 + tid;
+    const bool copy = r < p.rows && p.src[r] >= 0 && p.base[r] < found;
+    int total;
+    const int at = copies + block_scan(copy, lds, total);
+    if (copy) p.copies[at] = make_int4(p.src[r], p.fresh[p.base[r]], plan_row(p, r).rest, 0);
+    copies += total;
+  }
+  if (tid == 0) { p.found[0] = found; p.found[1] = copies; p.shortage[0] = needed - found; }
 }
 
-// grid (x, rows): x = 0 writes the row's table and its counts, every x copies its share of the row's partial page.  Rows beyond p.rows stand for the old
-// rows, whose references go.
-__global__ __launch_bounds__(256) void paged_fork_apply_kernel(const ForkParams p) {
-  const int tid = threadIdx.x;
-  if ((int)blockIdx.y >= p.rows) {
-    if (blockIdx.x > 0) return;
-    const int o = blockIdx.y - p.rows;
-    const int heirs = p.children[o];
-    const int cap = p.slots * (int)p.page.d;
-    const int n = clamp_int(p.lengths[o], 0, cap), full = (int)div_by(p.page, (uint32_t)n), rest = n - full * (int)p.page.d;
-    for (int j = tid; j < p.slots; j += 256) {
-      const int id = p.table[o * p.table_row + j];
-      if ((uint32_t)id >= (uint32_t)p.pages) continue;
-      int gain = -1;
-      if (j < full) gain += heirs;
-      else if (j == full && rest > 0 && heirs > 0 && p.refs[id] == 1) gain += 1;
-      if (gain != 0) atomicAdd(&p.new_refs[id], gain);
-    }
-    return;
+// 1024 16-byte pieces of a copy by one workgroup: four loads a thread in flight, then the stores.  at(i): where piece i lies within a page.
+template <typename At>
+__device__ __forceinline__ void copy_pieces(const char* from, char* to, uint32_t first, uint32_t end, At at) {
+  uint4 v[4];
+  uint64_t o[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t i = first + k * 256 + threadIdx.x;
+    o[k] = at(i < end ? i : end - 1);
+    v[k] = *reinterpret_cast<const uint4*>(from + o[k]);
   }
-  const int r = blockIdx.y;
-  const RowPlan w = plan_row(p, r);
-  const int src = p.src[r], base = p.base[r], found = p.found[0];
-  if (blockIdx.x == 0) {
-    for (int j = tid; j < p.slots; j += 256) {
-      int id = -1;
-      if (j < w.kept && !(j == w.full && src >= 0)) {
-        id = p.table[w.parent * p.table_row + j];
-        if ((uint32_t)id >= (uint32_t)p.pages) id = -1;
-      } else if (j < w.want || (j == w.full && src >= 0)) {
-        const int at = base + (src >= 0 ? j - w.full : j - w.kept);
-        if (at < found) {
-          id = p.fresh[at];
-          atomicAdd(&p.new_refs[id], 1);
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (first + k * 256 + threadIdx.x < end) *reinterpret_cast<uint4*>(to + o[k]) = v[k];
+}
+
+// One wave per new row writes its table, one per old row takes back its references, and all workgroups together walk the copies in stretches of 1024
+// pieces.  (With the copies cut by rows and blocks of a page the grid was mostly workgroups that found nothing: 16 us for 53 MB.)
+__global__ __launch_bounds__(256) void paged_fork_apply_kernel(const ForkParams p, uint32_t stretches, FastDiv per_copy) {
+  const int lane = threadIdx.x & 63, found = p.found[0];
+  for (int w = blockIdx.x * 4 + (threadIdx.x >> 6); w < p.rows + p.old_rows; w += gridDim.x * 4) {
+    if (w < p.rows) {
+      const RowPlan row = plan_row(p, w);
+      const int src = p.src[w], base = p.base[w];
+      for (int j = lane; j < p.slots; j += 64) {
+        int id = -1;
+        if (j < row.kept && !(j == row.full && src >= 0)) {
+          id = p.table[row.parent * p.table_row + j];
+          if ((uint32_t)id >= (uint32_t)p.pages) id = -1;
+        } else if (j < row.want || (j == row.full && src >= 0)) {
+          const int at = base + (src >= 0 ? j - row.full : j - row.kept);
+          if (at < found) {
+            id = p.fresh[at];
+            atomicAdd(&p.new_refs[id], 1);
+          }
         }
+        p.new_table[(int64_t)w * p.slots + j] = id;
       }
-      p.new_table[(int64_t)r * p.slots + j] = id;
+    } else {
+      const int o = w - p.rows, heirs = p.children[o];
+      const int cap = p.slots * (int)p.page.d;
+      const int n = clamp_int(p.lengths[o], 0, cap), full = (int)div_by(p.page, (uint32_t)n), rest = n - full * (int)p.page.d;
+      for (int j = lane; j < p.slots; j += 64) {
+        const int id = p.table[o * p.table_row + j];
+        if ((uint32_t)id >= (uint32_t)p.pages) continue;
+        int gain = -1;
+        if (j < full) gain += heirs;
+        else if (j == full && rest > 0 && heirs > 0 && p.refs[id] == 1) gain += 1;
+        if (gain != 0) atomicAdd(&p.new_refs[id], gain);
+      }
     }
   }
-  if (src < 0 || base >= found) return;
-  const int dst = p.fresh[base];
-  const char* from = p.pool + src * p.page_bytes;
-  char* to = p.pool + dst * p.page_bytes;
-  const int per = (int)(w.rest * p.row_bytes / 16);  // 16-byte pieces of a block's tokens
-  for (int b = blockIdx.x; b < p.blocks; b += gridDim.x)
-    for (int i = tid; i < per; i += 256)
-      *reinterpret_cast<uint4*>(to + b * p.block_bytes + i * 16) = *reinterpret_cast<const uint4*>(from + b * p.block_bytes + i * 16);
+  const uint32_t items = (uint32_t)p.found[1] * stretches;
+  for (uint32_t i = blockIdx.x; i < items; i += gridDim.x) {
+    const uint32_t k = div_by(per_copy, i);
+    const int4 c = p.copies[k];
+    const uint32_t per = (uint32_t)(c.z * p.row_bytes / 16), end = per * (uint32_t)p.blocks, first = (i - k * stretches) * 1024;  // pieces of a block's tokens, of all
+    if (first >= end) continue;
+    copy_pieces(p.pool + c.x * p.page_bytes, p.pool + c.y * p.page_bytes, first, end, [&](uint32_t x) {
+      const uint32_t b = x / per;
+      return (uint64_t)b * p.block_bytes + (x - b * per) * 16u;
+    });
+  }
 }
 
 struct CompactParams {
@@ -238,7 +265,7 @@ __global__ __launch_bounds__(1024) void paged_compact_plan_kernel(const CompactP
   if (blk == 0 && tid == 0) { p.live[0] = M; p.counts[p.nblk] = M - lowest; }
 }
 
-__global__ __launch_bounds__(256) void paged_compact_apply_kernel(const CompactParams p, int64_t pieces) {
+__global__ __launch_bounds__(256) void paged_compact_apply_kernel(const CompactParams p, uint32_t pieces, uint32_t stretches, FastDiv per_page) {
   const int M = p.live[0], moves = p.counts[p.nblk];
   const int64_t step = (int64_t)gridDim.x * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
   for (int64_t i = first; i < (int64_t)p.rows * p.slots; i += step) {
@@ -249,10 +276,10 @@ __global__ __launch_bounds__(256) void paged_compact_apply_kernel(const CompactP
     p.new_table[i] = id;
   }
   for (int64_t i = first; i < p.pages; i += step) p.new_refs[i] = i >= M ? 0 : p.refs[i] > 0 ? p.refs[i] : p.refs[p.src[p.rank[i]]];
-  for (int k = blockIdx.x; k < moves; k += gridDim.x) {
-    const char* from = p.pool + p.src[k] * p.page_bytes;
-    char* to = p.pool + p.dst[k] * p.page_bytes;
-    for (int64_t i = threadIdx.x; i < pieces; i += 256) *reinterpret_cast<uint4*>(to + i * 16) = *reinterpret_cast<const uint4*>(from + i * 16);
+  const uint32_t items = (uint32_t)moves * stretches;
+  for (uint32_t i = blockIdx.x; i < items; i += gridDim.x) {
+    const uint32_t k = div_by(per_page, i);
+    copy_pieces(p.pool + p.src[k] * p.page_bytes, p.pool + p.dst[k] * p.page_bytes, (i - k * stretches) * 1024, pieces, [](uint32_t x) { return (uint64_t)x * 16; });
   }
 }
 
@@ -270,7 +297,7 @@ static int64_t fork_fresh(int rows, int slots, int pages) {
 
 extern "C" int64_t mmamd_paged_fork_workspace(int old_rows, int rows, int slots, int pages) {
   MMAMD_CHECK_ARG(old_rows >= 0 && rows >= 0 && slots >= 1 && pages >= 1, MMAMD_E_BADARG, "mmamd_paged_fork_workspace: rows %d -> %d, slots %d, pages %d", old_rows, rows, slots, pages);
-  return 4 * (2 * up4(old_rows) + 2 * up4(rows) + up4(fork_fresh(rows, slots, pages)) + 4);
+  return 4 * (2 * up4(old_rows) + 2 * up4(rows) + 4 * (int64_t)rows + up4(fork_fresh(rows, slots, pages)) + 4);
 }
 
 extern "C" int mmamd_paged_fork(void* pool, int pages, int blocks, int page_size, int64_t row_bytes, const int32_t* table, int64_t table_row, const int32_t* lengths,
@@ -279,7 +306,8 @@ extern "C" int mmamd_paged_fork(void* pool, int pages, int blocks, int page_size
                                 mmamd_stream_t stream) {
   MMAMD_CHECK_ARG(pages >= 1 && blocks >= 1 && page_size >= 1 && slots >= 1 && old_rows >= 0 && rows >= 0, MMAMD_E_BADARG,
                   "mmamd_paged_fork: pages %d, blocks %d, page size %d, slots %d, rows %d -> %d", pages, blocks, page_size, slots, old_rows, rows);
-  MMAMD_CHECK_ARG((int64_t)slots * page_size <= 1 << 30 && (int64_t)rows + old_rows <= 65535 && (int64_t)rows * slots <= 0x7fffffffll && pages <= 0x7fffffff - 65536 && (int64_t)page_size * row_bytes <= 0x7fffffffll, MMAMD_E_UNSUPPORTED,
+  MMAMD_CHECK_ARG((int64_t)slots * page_size <= 1 << 30 && (int64_t)rows + old_rows <= 65535 && (int64_t)rows * slots <= 0x7fffffffll && pages <= 0x7fffffff - 65536 && (int64_t)page_size * row_bytes * blocks <= 0x7fffffffll &&
+                      (int64_t)rows * (((int64_t)page_size * row_bytes * blocks / 16 + 1023) / 1024) <= 0x7fffffffll, MMAMD_E_UNSUPPORTED,
                   "mmamd_paged_fork: %d slots of %d tokens, %d rows -> %d", slots, page_size, old_rows, rows);
   MMAMD_CHECK_ARG(pool != nullptr && refcounts != nullptr && new_refcounts != nullptr && shortage != nullptr && workspace != nullptr, MMAMD_E_BADARG, "mmamd_paged_fork: null argument");
   MMAMD_CHECK_ARG((old_rows == 0 || (table != nullptr && lengths != nullptr)) && (rows == 0 || (parents != nullptr && new_table != nullptr && new_lengths != nullptr)), MMAMD_E_BADARG,
@@ -297,6 +325,7 @@ extern "C" int mmamd_paged_fork(void* pool, int pages, int blocks, int page_size
   p.base = w; w += up4(rows);
   p.src = w; w += up4(rows);
   p.found = w; w += 4;
+  p.copies = reinterpret_cast<int4*>(w); w += 4 * (int64_t)rows;
   p.fresh = w;
   p.fresh_max = (int)fork_fresh(rows, slots, pages);
   p.table_row = table_row;
@@ -309,8 +338,11 @@ extern "C" int mmamd_paged_fork(void* pool, int pages, int blocks, int page_size
   paged_fork_plan_kernel<<<1 + copiers, 1024, 0, st>>>(p);
   if (int rc = launch_status("paged_fork plan")) return rc;
   if (rows + old_rows == 0) return 0;
-  const int gx = blocks < 64 ? blocks : 64;
-  paged_fork_apply_kernel<<<dim3(gx, rows + old_rows), 256, 0, st>>>(p);
+  const uint32_t stretches = (uint32_t)((p.page_bytes / 16 + 1023) / 1024);
+  int64_t grid = (int64_t)rows * stretches;  // no more than 8 workgroups a CU, and one for every four rows
+  if (grid > 2048) grid = 2048;
+  if (grid < (rows + old_rows + 3) / 4) grid = (rows + old_rows + 3) / 4;
+  paged_fork_apply_kernel<<<(unsigned)grid, 256, 0, st>>>(p, stretches, fast_div(stretches));
   return launch_status("paged_fork");
 }
 
@@ -322,7 +354,8 @@ extern "C" int64_t mmamd_paged_compact_workspace(int pages) {
 extern "C" int mmamd_paged_compact(void* pool, int pages, int64_t page_bytes, const int32_t* table, int64_t table_row, int rows, int slots, const int32_t* refcounts,
                                    int32_t* new_table, int32_t* new_refcounts, int32_t* live, void* workspace, int64_t workspace_bytes, mmamd_stream_t stream) {
   MMAMD_CHECK_ARG(pages >= 1 && rows >= 0 && slots >= 1 && page_bytes > 0, MMAMD_E_BADARG, "mmamd_paged_compact: pages %d of %lld bytes, %d rows of %d slots", pages, (long long)page_bytes, rows, slots);
-  MMAMD_CHECK_ARG(pages <= 0x7fffffff - 65536, MMAMD_E_UNSUPPORTED, "mmamd_paged_compact: %d pages", pages);
+  MMAMD_CHECK_ARG(pages <= 0x7fffffff - 65536 && page_bytes <= 0x7fffffffll && (int64_t)pages * ((page_bytes / 16 + 1023) / 1024) <= 0x7fffffffll, MMAMD_E_UNSUPPORTED,
+                  "mmamd_paged_compact: %d pages of %lld bytes", pages, (long long)page_bytes);
   MMAMD_CHECK_ARG(pool != nullptr && refcounts != nullptr && new_refcounts != nullptr && live != nullptr && workspace != nullptr && (rows == 0 || (table != nullptr && new_table != nullptr)),
                   MMAMD_E_BADARG, "mmamd_paged_compact: null argument");
   MMAMD_CHECK_ARG(aligned16(pool) && page_bytes % 16 == 0, MMAMD_E_ALIGN, "mmamd_paged_compact: the pool must be 16-byte aligned, with pages of whole 16-byte pieces");
@@ -342,6 +375,7 @@ extern "C" int mmamd_paged_compact(void* pool, int pages, int64_t page_bytes, co
   if (int rc = launch_status("paged_compact count")) return rc;
   paged_compact_plan_kernel<<<p.nblk, 1024, 0, st>>>(p);
   if (int rc = launch_status("paged_compact plan")) return rc;
-  paged_compact_apply_kernel<<<2048, 256, 0, st>>>(p, page_bytes / 16);
+  const uint32_t stretches = (uint32_t)((page_bytes / 16 + 1023) / 1024);
+  paged_compact_apply_kernel<<<2048, 256, 0, st>>>(p, (uint32_t)(page_bytes / 16), stretches, fast_div(stretches));
   return launch_status("paged_compact");
 }
