@@ -161,22 +161,21 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(const BeamParams p) {
 }
 
 // One workgroup per group.  A wave per beam joins the sums and merges the units' lists into the beam's `beams` best; the continuations of all beams then
-// count how many are better than they, which is their place.
+// count how many are better than they, which is their place.  Bound by its chain of dependent steps, so everything that can be loaded is loaded at once: a
+// row that was not scanned has whatever lay in the workspace, and does not use it.
 __global__ __launch_bounds__(512) void beam_join_kernel(const BeamParams p) {
+  __shared__ double total[kBeamMost * kBeamMost];  // of the continuations of all beams: beam * beams + place
   __shared__ double rank[kBeamMost * kBeamMost];
-  __shared__ float total[kBeamMost * kBeamMost];
   __shared__ uint32_t token[kBeamMost * kBeamMost];
-  __shared__ int place[kBeamMost];
+  __shared__ int better[kBeamMost * kBeamMost], place[kBeamMost], len[kBeamMost];
+  __shared__ bool fin[kBeamMost];
   const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, K = p.beams;
   for (int b = wave; b < K; b += blockDim.x >> 6) {
     const int row = g * K + b;
-    const bool fin = p.finished[row] != 0;
-    const double score = (double)p.scores[row];
     const int count = p.units * K;
     const uint2* list = p.unit_top + (int64_t)row * count;
     const float* um = p.unit_max + (int64_t)row * p.units;
     const double* us = p.unit_sum + (int64_t)row * p.units;
-    const bool on = !fin && score > -INFINITY;
     // up to four candidates a lane are kept in registers, more are read again for every place
     const bool few = count <= 256;
     float cv[4];
@@ -184,27 +183,29 @@ __global__ __launch_bounds__(512) void beam_join_kernel(const BeamParams p) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const int c = lane + j * 64;
-      const uint2 e = on && few && c < count ? list[c] : make_uint2(0xff800000u, 0xffffffffu);
+      const uint2 e = few && c < count ? list[c] : make_uint2(0xff800000u, 0xffffffffu);
       cv[j] = __uint_as_float(e.x);
       ci[j] = e.y;
     }
+    const float m0 = lane < p.units ? um[lane] : -INFINITY;
+    const double s0 = lane < p.units ? us[lane] : 0.0;
+    const bool done = p.finished[row] != 0;
+    const double score = (double)p.scores[row];
+    const int after = p.lengths[row] + (done ? 0 : 1);
     double lse = NAN;
-    if (on) {
-      float top = -INFINITY;
-      for (int u = lane; u < p.units; u += 64) top = fmaxf(top, um[u]);
+    if (!done && score > -INFINITY) {
+      float top = m0;
+      for (int u = lane + 64; u < p.units; u += 64) top = fmaxf(top, um[u]);
       top = dpp_max(top);
-      double sum = 0.0;
-      for (int u = lane; u < p.units; u += 64) sum += um[u] > -INFINITY ? us[u] * exp((double)um[u] - (double)top) : us[u];
+      double sum = m0 > -INFINITY ? s0 * exp((double)m0 - (double)top) : s0;
+      for (int u = lane + 64; u < p.units; u += 64) sum += um[u] > -INFINITY ? us[u] * exp((double)um[u] - (double)top) : us[u];
 #pragma unroll
       for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
       lse = (double)top + log(sum);
     }
-    const int len = p.lengths[row] + (fin ? 0 : 1);
-    const double base = (double)(len > 1 ? len : 1);
-    const double div = p.penalty == 0.0 ? 1.0 : p.penalty == 1.0 ? base : pow(base, p.penalty);
     if (lse > -INFINITY && lse < INFINITY) {
-      float v0 = INFINITY;
-      uint32_t i0 = 0;
+      float v0 = INFINITY, mine = -INFINITY;  // the last one taken; lane k's: the k-th
+      uint32_t i0 = 0, word = 0xffffffffu;
       int found = 0;
       for (; found < K; ++found) {
         float bv = -INFINITY;
@@ -235,61 +236,62 @@ __global__ __launch_bounds__(512) void beam_join_kernel(const BeamParams p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (ci[j] == low) { cv[j] = -INFINITY; ci[j] = 0xffffffffu; }
-        if (lane == 0) {
-          const double t = score + ((double)best - lse);
-          rank[b * K + found] = t / div;
-          total[b * K + found] = (float)t;
-          token[b * K + found] = low;
-        }
+        if (lane == found) { mine = best; word = low; }
+      }
+      if (lane < K) {
+        total[b * K + lane] = lane < found ? score + ((double)mine - lse) : -INFINITY;
+        token[b * K + lane] = word;
       }
       if (found < K && lane == 0) {  // all finite ones are listed: the first words that are not, at -inf
         uint32_t t = 0;
         for (int k = found; k < K; ++k, ++t) {
           for (int d = 0; d < found; ++d)
             if (token[b * K + d] == t) { ++t; d = -1; }
-          rank[b * K + k] = -INFINITY;
-          total[b * K + k] = -INFINITY;
           token[b * K + k] = t < (uint32_t)p.vocab ? t : 0xffffffffu;
         }
       }
     } else if (lane < K) {
       // a finished beam goes on as it is; every other continuation of it, and all of a dead beam, tie at -inf: the first ones of them
       const int eos = (int)p.eos;
-      const bool alive = fin && score > -INFINITY;
+      const bool alive = done && score > -INFINITY;
       const int t = !alive ? lane : lane == 0 ? eos : (lane - 1 < eos ? lane - 1 : lane);
-      const double own = alive && lane == 0 ? score : -INFINITY;
-      rank[b * K + lane] = own / div;
-      total[b * K + lane] = (float)own;
+      total[b * K + lane] = alive && lane == 0 ? score : -INFINITY;
       token[b * K + lane] = t < p.vocab ? (uint32_t)t : 0xffffffffu;
     }
+    if (lane < K) {
+      const double base = (double)(after > 1 ? after : 1);
+      rank[b * K + lane] = p.penalty == 0.0 ? total[b * K + lane] : total[b * K + lane] / (p.penalty == 1.0 ? base : pow(base, p.penalty));
+    }
+    if (lane < K) better[b * K + lane] = 0;
+    if (lane == 0) { fin[b] = done; len[b] = after; }
   }
   __syncthreads();
-  for (int c = tid; c < K * K; c += blockDim.x) {
-    if (token[c] == 0xffffffffu) continue;  // (a vocabulary smaller than the beams)
-    const double r = rank[c];
-    const int64_t flat = (int64_t)(c / K) * p.vocab + token[c];
-    int better = 0, d = 0;
-    for (int b = 0; b < K; ++b)
-      for (int k = 0; k < K; ++k, ++d)
-        better += token[d] != 0xffffffffu && (rank[d] > r || (rank[d] == r && (int64_t)b * p.vocab + token[d] < flat));
-    if (better < K) place[better] = c;
+  // every pair of continuations is compared by a thread of its own
+  const int all = K * K;
+  for (int x = tid; x < all * all; x += blockDim.x) {
+    const int c = x / all, d = x - c * all;
+    if (token[d] == 0xffffffffu) continue;               // (a vocabulary smaller than the beams)
+    const double r = rank[c], q = rank[d];
+    if (q > r || (q == r && (d / K < c / K || (d / K == c / K && token[d] < token[c])))) atomicAdd(&better[c], 1);
   }
+  __syncthreads();
+  for (int c = tid; c < all; c += blockDim.x)
+    if (token[c] != 0xffffffffu && better[c] < K) place[better[c]] = c;
   __syncthreads();
   for (int k = tid; k < K; k += blockDim.x) {
-    const int c = place[k], row = g * K + c / K, to = g * K + k;
-    const bool fin = p.finished[row] != 0;
-    p.out_scores[to] = total[c];
-    p.out_lengths[to] = p.lengths[row] + (fin ? 0 : 1);
-    p.out_finished[to] = fin || token[c] == (uint32_t)p.eos;
+    const int c = place[k], b = c / K, to = g * K + k;
+    p.out_scores[to] = (float)total[c];
+    p.out_lengths[to] = len[b];
+    p.out_finished[to] = fin[b] || token[c] == (uint32_t)p.eos;
     p.out_tokens[to] = token[c];
-    p.out_parents[to] = row;
+    p.out_parents[to] = g * K + b;
   }
   if (p.out_sequences == nullptr) return;
-  for (int64_t i = tid; i < (int64_t)K * p.tokens; i += blockDim.x) {
-    const int k = (int)(i / p.tokens), t = (int)(i - (int64_t)k * p.tokens);
-    const int c = place[k], row = g * K + c / K;
-    const bool put = p.finished[row] == 0 && t == p.lengths[row];
-    p.out_sequences[(int64_t)g * K * p.tokens + i] = put ? (int64_t)token[c] : p.sequences[(int64_t)row * p.tokens + t];
+  for (int k = wave; k < K; k += blockDim.x >> 6) {
+    const int c = place[k], b = c / K, at = fin[b] ? -1 : len[b] - 1;
+    const int64_t* from = p.sequences + (int64_t)(g * K + b) * p.tokens;
+    int64_t* to = p.out_sequences + (int64_t)(g * K + k) * p.tokens;
+    for (int t = lane; t < p.tokens; t += 64) to[t] = t == at ? (int64_t)token[c] : from[t];
   }
 }
 

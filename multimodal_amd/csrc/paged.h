@@ -25,6 +25,12 @@ __host__ __device__ __forceinline__ uint32_t div_by(const FastDiv& f, uint32_t n
   return (t + ((n - t) >> f.sh1)) >> f.sh2;
 }
 
+// 16-byte pieces past the caches.  A copy's stores: left in the L2, its lines are written back when the kernel ends, which waits for them (36 MB moved within a
+// pool: 21.7 us a call with ordinary stores, 11.3 with these; 240 MB: 64.0 and 48.6).
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
+__device__ __forceinline__ uint4 load_past(const void* at) { return __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at))); }
+__device__ __forceinline__ void store_past(void* at, const uint4& v) { __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), reinterpret_cast<u32x4*>(at)); }
+
 __device__ __forceinline__ int clamp_int(int v, int lo, int hi) { return v < lo ? lo : (v > hi ? hi : v); }
 
 }  // namespace mmamd

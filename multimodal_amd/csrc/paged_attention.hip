@@ -56,13 +56,19 @@ __device__ __forceinline__ f32x4 mma16<float>(const uint4& a, const uint4& b, f3
   return c;
 }
 
+template <bool STREAM>
+__device__ __forceinline__ uint4 load_piece(const char* at) {
+  if constexpr (STREAM) return load_past(at);
+  else return *reinterpret_cast<const uint4*>(at);
+}
+
 // One workgroup: up to 16 query heads of one key head of one row over one split of the row's tokens, so that the cache is read once whatever the group
 // is.  The four waves take the split's tiles (32 tokens in bf16, 16 in fp32) in turn, each with its own running maximum, sum and output:
 //   scores [token, head] = K . q: the tile's keys go from memory to the registers of a 16 x 16 product as they lie (lane = token, 4 lanes share a row);
 //   out [dim, head] += V^T . weights: the values go through LDS for their columns, the weights are where the first product left them.
 // A pass over a tile ends with the loads of the next one in flight, and the page numbers of the one after.  fp32 runs on the fp32 matrix instruction.
 // bf16 weights are split in two bf16 parts (2^-16 of a weight is lost): in one part they would lose as much as the output's own rounding.
-template <typename T, int D>
+template <typename T, int D, bool STREAM>
 __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const PagedAttnParams p) {
   constexpr int TOK = sizeof(T) == 2 ? 32 : 16;      // tokens of a tile
   constexpr int NT = TOK / 16;
@@ -117,13 +123,13 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const PagedAttnParam
     for (int u = 0; u < NT; ++u) {
       const int64_t o = (int64_t)(((uint64_t)(uint32_t)__shfl(khi, u * 16 + l15) << 32) | (uint32_t)__shfl(klo, u * 16 + l15));
 #pragma unroll
-      for (int i = 0; i < KP; ++i) kr[u][i] = *reinterpret_cast<const uint4*>(keys + o + (i * 4 + quarter) * 16);
+      for (int i = 0; i < KP; ++i) kr[u][i] = load_piece<STREAM>(keys + o + (i * 4 + quarter) * 16);
     }
 #pragma unroll
     for (int i = 0; i < VP; ++i) {
       const int piece = i * 64 + lane, tok = piece / PIECES, x = piece - tok * PIECES;
       const int64_t o = (int64_t)(((uint64_t)(uint32_t)__shfl(vhi, tok) << 32) | (uint32_t)__shfl(vlo, tok));
-      vr[i] = *reinterpret_cast<const uint4*>(values + o + x * 16);
+      vr[i] = load_piece<STREAM>(values + o + x * 16);
     }
   };
 
@@ -248,7 +254,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const PagedAttnParam
       v = fmaf(red[(w * 16 + g) * RROW + d], fac, v);
     }
     const int64_t rh = (int64_t)row * p.heads + h0 + g;
-    if (p.splits == 1) {
+    if (n <= chunk) {  // one split holds the whole row
       reinterpret_cast<T*>(p.out)[rh * D + d] = (T)(ls == 0.f ? 0.f : v / ls);
     } else {
       const int64_t at = rh * p.splits + split;
@@ -268,10 +274,12 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
   const int h = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   int pos;
   const int n = row_tokens(p, row, pos);
-  const int chunk = row_chunk(p, n);
-  const int used = n > 0 ? (n + chunk - 1) / chunk : 1;
   const int64_t rh = (int64_t)row * p.heads + h;
-  const float2 ml = tid < used ? reinterpret_cast<const float2*>(p.ws + (int64_t)p.rows * p.heads * p.splits * D)[rh * p.splits + tid] : make_float2(-3.402823466e38f, 0.f);
+  float2 ml = tid < p.splits ? reinterpret_cast<const float2*>(p.ws + (int64_t)p.rows * p.heads * p.splits * D)[rh * p.splits + tid] : make_float2(0.f, 0.f);
+  const int chunk = row_chunk(p, n);
+  if (n <= chunk) return;                               // a single split has written its output
+  const int used = (n + chunk - 1) / chunk;
+  if (tid >= used) ml = make_float2(-3.402823466e38f, 0.f);  // (what nobody wrote)
   float top = wave_max(ml.x);
   if (lane == 0) red[wave] = top;
   __syncthreads();
@@ -313,11 +321,18 @@ static int paged_splits(int rows, int heads, int kv_heads, int64_t capacity) {
   return s < 1 ? 1 : (int)s;
 }
 
+// A pool of this size or less is read through the caches as usual, a larger one past them.  Us a call, as usual / past them: 1.07 GB 196.6 / 181.1; 322 MB
+// 69.6 / 70.4; 50 MB whose pages eight rows share 110 / 121.
+constexpr int64_t kStreamBytes = 512ll << 20;
+
 template <typename T, int D>
 static int launch_paged_attn(PagedAttnParams& p, hipStream_t st) {
   p.sub = (p.group + 15) / 16;
   p.min_chunk = 128;
-  paged_attn_kernel<T, D><<<dim3(p.splits, p.kv_heads * p.sub, p.rows), 256, 0, st>>>(p);
+  const dim3 grid(p.splits, p.kv_heads * p.sub, p.rows);
+  const int64_t pool = 2ll * p.pages * p.kv_heads * p.page.d * D * (int64_t)sizeof(T);
+  if (pool > kStreamBytes) paged_attn_kernel<T, D, true><<<grid, 256, 0, st>>>(p);
+  else paged_attn_kernel<T, D, false><<<grid, 256, 0, st>>>(p);
   if (int rc = launch_status("paged_attention")) return rc;
   if (p.splits > 1) {
     paged_join_kernel<T, D><<<dim3(p.heads, p.rows), 256, 0, st>>>(p);
@@ -344,16 +359,24 @@ struct PagedAppendParams {
   FastDiv page, per_token, per_head;
 };
 
-// One 16-byte piece per thread and step; consecutive threads walk the pieces of a head, the heads and the tokens, so both sides see whole rows.
+// Four 16-byte pieces a thread, all loaded before the first is stored; consecutive threads walk the pieces of a head, the heads and the tokens, so both sides
+// see whole rows.
 __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendParams p) {
   const int row = blockIdx.y;
   int count = p.counts != nullptr ? p.counts[row] : p.tokens;
   count = count < p.tokens ? count : p.tokens;
   const int64_t start = p.start[row];
   const uint32_t total = count > 0 ? (uint32_t)count * p.per_token.d : 0u;
-  for (uint32_t i = blockIdx.x * 256u + threadIdx.x; i < total; i += gridDim.x * 256u) {
+  const uint32_t first = blockIdx.x * 1024u + threadIdx.x;
+  uint4 piece[4];
+  char* to[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t i = first + k * 256u;
+    to[k] = nullptr;
+    if (i >= total) continue;
     const uint32_t j = div_by(p.per_token, i), x = i - j * p.per_token.d;   // token, place within it
-    const uint32_t hv = div_by(p.per_head, x), piece = x - hv * p.per_head.d;
+    const uint32_t hv = div_by(p.per_head, x), at = (x - hv * p.per_head.d) * 16u;
     const bool val = hv >= (uint32_t)p.kv_heads;
     const int h = (int)(val ? hv - p.kv_heads : hv);
     const int64_t t = start + j;
@@ -363,10 +386,13 @@ __global__ __launch_bounds__(256) void paged_append_kernel(const PagedAppendPara
     if ((uint32_t)id >= (uint32_t)p.pages) continue;
     const char* src = val ? reinterpret_cast<const char*>(p.v) + row * p.v_row + j * p.v_token + h * p.v_head
                           : reinterpret_cast<const char*>(p.k) + row * p.k_row + j * p.k_token + h * p.k_head;
-    char* dst = val ? reinterpret_cast<char*>(p.values) + id * p.value_page + h * p.value_head + off * p.value_token
-                    : reinterpret_cast<char*>(p.keys) + id * p.key_page + h * p.key_head + off * p.key_token;
-    *reinterpret_cast<uint4*>(dst + piece * 16) = *reinterpret_cast<const uint4*>(src + piece * 16);
+    to[k] = (val ? reinterpret_cast<char*>(p.values) + id * p.value_page + h * p.value_head + off * p.value_token
+                 : reinterpret_cast<char*>(p.keys) + id * p.key_page + h * p.key_head + off * p.key_token) + at;
+    piece[k] = *reinterpret_cast<const uint4*>(src + at);
   }
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    if (to[k] != nullptr) store_past(to[k], piece[k]);
 }
 
 static bool good_stride(int64_t s, int size) { return s >= 0 && (s * size) % 16 == 0; }

@@ -64,8 +64,9 @@ __device__ __forceinline__ int block_scan(int v, int* lds, int& total) {
   return before + inc - v;
 }
 
-// Workgroup 0 plans: the lowest child of every parent, the pages each new row needs (numbered over the rows in order), the lowest free pages.  The
-// others copy the counts, which paged_fork_apply_kernel then changes by what the tables gain and lose.
+// Workgroup 0 plans: the lowest child of every parent, the pages each new row needs (numbered over the rows in order), the lowest free pages, the
+// copies.  The others copy the counts, which paged_fork_apply_kernel then changes by what the tables gain and lose.  Bound by its chain of dependent loads.
+constexpr int kForkOld = 4096;  // old rows whose children are counted in LDS
 __global__ __launch_bounds__(1024) void paged_fork_plan_kernel(const ForkParams p) {
   const int tid = threadIdx.x;
   if (blockIdx.x > 0) {
@@ -73,15 +74,29 @@ __global__ __launch_bounds__(1024) void paged_fork_plan_kernel(const ForkParams 
     return;
   }
   __shared__ int lds[16];
-  for (int i = tid; i < p.old_rows; i += 1024) { p.first[i] = 0x7fffffff; p.children[i] = 0; }
+  __shared__ int near_first[kForkOld], near_children[kForkOld];
+  int* const first = p.old_rows <= kForkOld ? near_first : p.first;
+  int* const children = p.old_rows <= kForkOld ? near_children : p.children;
+  int ahead[4];                                      // counts of the next 4096 pages
+  auto look = [&](int i0) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int i = i0 + tid * 4 + k;
+      ahead[k] = i < p.pages ? p.refs[i] : 1;
+    }
+  };
+  look(0);
+  for (int i = tid; i < p.old_rows; i += 1024) { first[i] = 0x7fffffff; children[i] = 0; }
   __threadfence_block();
   __syncthreads();
   for (int r = tid; r < p.rows; r += 1024) {
     const int parent = p.parents[r];
-    if ((uint32_t)parent < (uint32_t)p.old_rows) { atomicMin(&p.first[parent], r); atomicAdd(&p.children[parent], 1); }
+    if ((uint32_t)parent < (uint32_t)p.old_rows) { atomicMin(&first[parent], r); atomicAdd(&children[parent], 1); }
   }
   __threadfence_block();
   __syncthreads();
+  if (p.old_rows <= kForkOld)
+    for (int i = tid; i < p.old_rows; i += 1024) p.children[i] = children[i];
   int needed = 0;
   for (int r0 = 0; r0 < p.rows; r0 += 1024) {
     const int r = r0 + tid;
@@ -91,7 +106,8 @@ __global__ __launch_bounds__(1024) void paged_fork_plan_kernel(const ForkParams 
       need = w.want > w.kept ? w.want - w.kept : 0;
       if (w.rest > 0) {
         const int id = p.table[w.parent * p.table_row + w.full];
-        if ((uint32_t)id < (uint32_t)p.pages && !(__hip_atomic_load(&p.first[w.parent], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == r && p.refs[id] == 1)) {
+        // (the loads past the first-level cache: for more old rows the minima were made by atomics beyond it)
+        if ((uint32_t)id < (uint32_t)p.pages && !(__hip_atomic_load(&first[w.parent], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == r && p.refs[id] == 1)) {
           src = id;
           ++need;
         }
@@ -108,10 +124,10 @@ __global__ __launch_bounds__(1024) void paged_fork_plan_kernel(const ForkParams 
     int c[4], mine = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int i = i0 + tid * 4 + k;
-      c[k] = i < p.pages && p.refs[i] <= 0;
+      c[k] = ahead[k] <= 0;
       mine += c[k];
     }
+    if (i0 + 4096 < p.pages) look(i0 + 4096);
     int total;
     int at = found + block_scan(mine, lds, total);
 #pragma unroll
@@ -136,8 +152,10 @@ __global__ __launch_bounds__(1024) void paged_fork_plan_kernel(const ForkParams 
   if (tid == 0) { p.found[0] = found; p.found[1] = copies; p.shortage[0] = needed - found; }
 }
 
-// 1024 16-byte pieces of a copy by one workgroup: four loads a thread in flight, then the stores.  at(i): where piece i lies within a page.
-template <typename At>
+// 1024 16-byte pieces of a copy by one workgroup: four loads a thread in flight, then the stores.  at(i): where piece i lies within a page.  OLD: nobody
+// has touched the source lately, it is read past the caches as well (a large compaction 219 us against 228; a fork's pages were just written: 65 us
+// against 49).
+template <bool OLD, typename At>
 __device__ __forceinline__ void copy_pieces(const char* from, char* to, uint32_t first, uint32_t end, At at) {
   uint4 v[4];
   uint64_t o[4];
@@ -145,59 +163,62 @@ __device__ __forceinline__ void copy_pieces(const char* from, char* to, uint32_t
   for (int k = 0; k < 4; ++k) {
     const uint32_t i = first + k * 256 + threadIdx.x;
     o[k] = at(i < end ? i : end - 1);
-    v[k] = *reinterpret_cast<const uint4*>(from + o[k]);
+    if constexpr (OLD) v[k] = load_past(from + o[k]);
+    else v[k] = *reinterpret_cast<const uint4*>(from + o[k]);
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k)
-    if (first + k * 256 + threadIdx.x < end) *reinterpret_cast<uint4*>(to + o[k]) = v[k];
+    if (first + k * 256 + threadIdx.x < end) store_past(to + o[k], v[k]);
 }
 
-// One wave per new row writes its table, one per old row takes back its references, and all workgroups together walk the copies in stretches of 1024
-// pieces.  (With the copies cut by rows and blocks of a page the grid was mostly workgroups that found nothing: 16 us for 53 MB.)
-__global__ __launch_bounds__(256) void paged_fork_apply_kernel(const ForkParams p, uint32_t stretches, FastDiv per_copy) {
-  const int lane = threadIdx.x & 63, found = p.found[0];
-  for (int w = blockIdx.x * 4 + (threadIdx.x >> 6); w < p.rows + p.old_rows; w += gridDim.x * 4) {
-    if (w < p.rows) {
-      const RowPlan row = plan_row(p, w);
-      const int src = p.src[w], base = p.base[w];
-      for (int j = lane; j < p.slots; j += 64) {
-        int id = -1;
-        if (j < row.kept && !(j == row.full && src >= 0)) {
-          id = p.table[row.parent * p.table_row + j];
-          if ((uint32_t)id >= (uint32_t)p.pages) id = -1;
-        } else if (j < row.want || (j == row.full && src >= 0)) {
-          const int at = base + (src >= 0 ? j - row.full : j - row.kept);
-          if (at < found) {
-            id = p.fresh[at];
-            atomicAdd(&p.new_refs[id], 1);
-          }
-        }
-        p.new_table[(int64_t)w * p.slots + j] = id;
-      }
-    } else {
-      const int o = w - p.rows, heirs = p.children[o];
-      const int cap = p.slots * (int)p.page.d;
-      const int n = clamp_int(p.lengths[o], 0, cap), full = (int)div_by(p.page, (uint32_t)n), rest = n - full * (int)p.page.d;
-      for (int j = lane; j < p.slots; j += 64) {
-        const int id = p.table[o * p.table_row + j];
-        if ((uint32_t)id >= (uint32_t)p.pages) continue;
-        int gain = -1;
-        if (j < full) gain += heirs;
-        else if (j == full && rest > 0 && heirs > 0 && p.refs[id] == 1) gain += 1;
-        if (gain != 0) atomicAdd(&p.new_refs[id], gain);
-      }
-    }
+// The first rows * share workgroups move data, `share` of them a copy, which split its pieces evenly: the copies differ in their tokens, so cut into stretches of
+// one length they were mostly empty or a second round.  The others write tables: one wave per new row, and one per old row that takes back its references.
+__global__ __launch_bounds__(256) void paged_fork_apply_kernel(const ForkParams p, uint32_t share, FastDiv per_copy) {
+  const uint32_t copiers = (uint32_t)p.rows * share;
+  if (blockIdx.x < copiers) {
+    const uint32_t k = div_by(per_copy, blockIdx.x), part = blockIdx.x - k * share;
+    const int4 c = p.copies[k];                        // (loaded beside the number of copies; behind it, whatever lay there)
+    if ((int)k >= p.found[1]) return;
+    const uint32_t per = (uint32_t)(c.z * p.row_bytes / 16), all = per * (uint32_t)p.blocks;  // pieces of a block's tokens, of the copy
+    const uint32_t mine = (all + share - 1) / share, end = (part + 1) * mine < all ? (part + 1) * mine : all;
+    for (uint32_t first = part * mine; first < end; first += 1024)
+      copy_pieces<false>(p.pool + c.x * p.page_bytes, p.pool + c.y * p.page_bytes, first, end, [&](uint32_t x) {
+        const uint32_t b = x / per;
+        return (uint64_t)b * p.block_bytes + (x - b * per) * 16u;
+      });
+    return;
   }
-  const uint32_t items = (uint32_t)p.found[1] * stretches;
-  for (uint32_t i = blockIdx.x; i < items; i += gridDim.x) {
-    const uint32_t k = div_by(per_copy, i);
-    const int4 c = p.copies[k];
-    const uint32_t per = (uint32_t)(c.z * p.row_bytes / 16), end = per * (uint32_t)p.blocks, first = (i - k * stretches) * 1024;  // pieces of a block's tokens, of all
-    if (first >= end) continue;
-    copy_pieces(p.pool + c.x * p.page_bytes, p.pool + c.y * p.page_bytes, first, end, [&](uint32_t x) {
-      const uint32_t b = x / per;
-      return (uint64_t)b * p.block_bytes + (x - b * per) * 16u;
-    });
+  const int found = p.found[0];
+  const int lane = threadIdx.x & 63, w = (int)(blockIdx.x - copiers) * 4 + (threadIdx.x >> 6);
+  if (w < p.rows) {
+    const RowPlan row = plan_row(p, w);
+    const int src = p.src[w], base = p.base[w];
+    for (int j = lane; j < p.slots; j += 64) {
+      int id = -1;
+      if (j < row.kept && !(j == row.full && src >= 0)) {
+        id = p.table[row.parent * p.table_row + j];
+        if ((uint32_t)id >= (uint32_t)p.pages) id = -1;
+      } else if (j < row.want || (j == row.full && src >= 0)) {
+        const int at = base + (src >= 0 ? j - row.full : j - row.kept);
+        if (at < found) {
+          id = p.fresh[at];
+          atomicAdd(&p.new_refs[id], 1);
+        }
+      }
+      p.new_table[(int64_t)w * p.slots + j] = id;
+    }
+  } else if (w < p.rows + p.old_rows) {
+    const int o = w - p.rows, heirs = p.children[o];
+    const int cap = p.slots * (int)p.page.d;
+    const int n = clamp_int(p.lengths[o], 0, cap), full = (int)div_by(p.page, (uint32_t)n), rest = n - full * (int)p.page.d;
+    for (int j = lane; j < p.slots; j += 64) {
+      const int id = p.table[o * p.table_row + j];
+      if ((uint32_t)id >= (uint32_t)p.pages) continue;
+      int gain = -1;
+      if (j < full) gain += heirs;
+      else if (j == full && rest > 0 && heirs > 0 && p.refs[id] == 1) gain += 1;
+      if (gain != 0) atomicAdd(&p.new_refs[id], gain);
+    }
   }
 }
 
@@ -205,7 +226,8 @@ struct CompactParams {
   char* pool;
   const int32_t *table, *refs;
   int32_t *new_table, *new_refs, *live;
-  int32_t *counts, *rank, *src, *dst;  // workspace: live pages per block, per page, moved pages
+  int32_t *moves, *counts, *rank;              // workspace: how many pages move, live pages per workgroup, a number per page
+  int2* moved;                                 // from page, to page
   int64_t table_row, page_bytes;
   int rows, slots, pages, nblk;
 };
@@ -219,68 +241,88 @@ __global__ __launch_bounds__(1024) void paged_compact_count_kernel(const Compact
   if (threadIdx.x == 0) p.counts[blockIdx.x] = total;
 }
 
-// With M live pages: the k-th live page from M on moves to the k-th free place before M.  Lists both, and numbers the movers.
+// With M live pages: the k-th live page from M on moves to the k-th free place before M.  Lists both, and numbers the movers and the places.  ALONE: every
+// workgroup counts the whole pool itself, which is one launch less and a few loads a thread for a small pool.
+template <bool ALONE>
 __global__ __launch_bounds__(1024) void paged_compact_plan_kernel(const CompactParams p) {
   __shared__ int lds[16];
-  __shared__ int sums[2];
+  __shared__ int sums[1];
   const int tid = threadIdx.x, blk = blockIdx.x;
-  int all = 0, before = 0;
-  for (int b0 = 0; b0 < p.nblk; b0 += 1024) {
-    const int b = b0 + tid;
-    const int c = b < p.nblk ? p.counts[b] : 0;
-    int total;
-    const int ex = block_scan(c, lds, total);
-    if (b == blk) sums[0] = before + ex;
-    all += total;
-    before += total;
-  }
-  __syncthreads();
-  const int mine = sums[0];                     // live pages before this workgroup's
-  const int M = all;
   const int i = blk * kCompactPer + tid;
   const bool live = i < p.pages && p.refs[i] > 0;
-  int total;
-  const int l = mine + block_scan(live, lds, total);   // live pages before page i
-  // live pages before M: from the back, M minus the ones from M on; counted by the workgroup that holds page M, and by nobody where M = pages
-  const int mb = M / kCompactPer;
-  int lowest = 0;
-  for (int b0 = 0; b0 < mb; b0 += 1024) {
-    const int b = b0 + tid;
-    int t;
-    block_scan(b < mb ? p.counts[b] : 0, lds, t);
-    lowest += t;
+  int M = 0, mine = 0;                                 // live pages, and those before this workgroup's
+  if constexpr (ALONE) {
+    int all = 0, before = 0;
+    for (int x = tid; x < p.pages; x += 1024) {
+      const int c = p.refs[x] > 0;
+      all += c;
+      before += x < blk * kCompactPer ? c : 0;
+    }
+    block_scan(all, lds, M);
+    block_scan(before, lds, mine);
+  } else {
+    for (int b0 = 0; b0 < p.nblk; b0 += 1024) {
+      const int b = b0 + tid;
+      int total;
+      const int ex = block_scan(b < p.nblk ? p.counts[b] : 0, lds, total);
+      if (b == blk) sums[0] = M + ex;
+      M += total;
+    }
+    __syncthreads();
+    mine = sums[0];
   }
-  {
+  int total, lowest = 0;                               // lowest: live pages before M
+  const int l = mine + block_scan(live, lds, total);   // live pages before page i
+  if constexpr (ALONE) {
+    int c = 0;
+    for (int x = tid; x < M; x += 1024) c += p.refs[x] > 0;
+    block_scan(c, lds, lowest);
+  } else {
+    const int mb = M / kCompactPer;
+    for (int b0 = 0; b0 < mb; b0 += 1024) {
+      const int b = b0 + tid;
+      int t;
+      block_scan(b < mb ? p.counts[b] : 0, lds, t);
+      lowest += t;
+    }
     const int x = mb * kCompactPer + tid;
     int t;
     block_scan(x < M && x < p.pages && p.refs[x] > 0, lds, t);
     lowest += t;
   }
   if (i < p.pages) {
-    int rank = 0;  // of a mover among the movers, of a hole among the holes
-    if (live && i >= M) { rank = l - lowest; p.src[rank] = i; }
-    else if (!live && i < M) { rank = i - l; p.dst[rank] = i; }
+    int rank = 0;
+    if (live && i >= M) { rank = l - lowest; p.moved[rank].x = i; }
+    else if (!live && i < M) { rank = i - l; p.moved[rank].y = i; }
     p.rank[i] = rank;
   }
-  if (blk == 0 && tid == 0) { p.live[0] = M; p.counts[p.nblk] = M - lowest; }
+  if (blk == 0 && tid == 0) { p.live[0] = M; p.moves[0] = M - lowest; }
 }
 
-__global__ __launch_bounds__(256) void paged_compact_apply_kernel(const CompactParams p, uint32_t pieces, uint32_t stretches, FastDiv per_page) {
-  const int M = p.live[0], moves = p.counts[p.nblk];
-  const int64_t step = (int64_t)gridDim.x * 256, first = (int64_t)blockIdx.x * 256 + threadIdx.x;
+// The first `copiers` workgroups walk the moved pages in stretches of 1024 pieces, the others rewrite the table and the counts.
+__global__ __launch_bounds__(256) void paged_compact_apply_kernel(const CompactParams p, uint32_t pieces, uint32_t stretches, FastDiv per_page, uint32_t copiers) {
+  if (blockIdx.x < copiers) {
+    uint32_t k = div_by(per_page, blockIdx.x);
+    int2 m = p.moved[k];                               // (loaded beside the number of moves; behind it, whatever lay there)
+    const uint32_t items = (uint32_t)p.moves[0] * stretches;
+    for (uint32_t i = blockIdx.x; i < items;) {
+      copy_pieces<true>(p.pool + m.x * p.page_bytes, p.pool + m.y * p.page_bytes, (i - k * stretches) * 1024, pieces, [](uint32_t x) { return (uint64_t)x * 16; });
+      i += copiers;
+      k = div_by(per_page, i);
+      if (i < items) m = p.moved[k];
+    }
+    return;
+  }
+  const int M = p.live[0];
+  const int64_t step = (int64_t)(gridDim.x - copiers) * 256, first = (int64_t)(blockIdx.x - copiers) * 256 + threadIdx.x;
   for (int64_t i = first; i < (int64_t)p.rows * p.slots; i += step) {
     const int r = (int)(i / p.slots), j = (int)(i - (int64_t)r * p.slots);
     int id = p.table[r * p.table_row + j];
     if ((uint32_t)id >= (uint32_t)p.pages || p.refs[id] <= 0) id = -1;
-    else if (id >= M) id = p.dst[p.rank[id]];
+    else if (id >= M) id = p.moved[p.rank[id]].y;
     p.new_table[i] = id;
   }
-  for (int64_t i = first; i < p.pages; i += step) p.new_refs[i] = i >= M ? 0 : p.refs[i] > 0 ? p.refs[i] : p.refs[p.src[p.rank[i]]];
-  const uint32_t items = (uint32_t)moves * stretches;
-  for (uint32_t i = blockIdx.x; i < items; i += gridDim.x) {
-    const uint32_t k = div_by(per_page, i);
-    copy_pieces(p.pool + p.src[k] * p.page_bytes, p.pool + p.dst[k] * p.page_bytes, (i - k * stretches) * 1024, pieces, [](uint32_t x) { return (uint64_t)x * 16; });
-  }
+  for (int64_t i = first; i < p.pages; i += step) p.new_refs[i] = i >= M ? 0 : p.refs[i] > 0 ? p.refs[i] : p.refs[p.moved[p.rank[i]].x];
 }
 
 }  // namespace mmamd
@@ -306,8 +348,7 @@ extern "C" int mmamd_paged_fork(void* pool, int pages, int blocks, int page_size
                                 mmamd_stream_t stream) {
   MMAMD_CHECK_ARG(pages >= 1 && blocks >= 1 && page_size >= 1 && slots >= 1 && old_rows >= 0 && rows >= 0, MMAMD_E_BADARG,
                   "mmamd_paged_fork: pages %d, blocks %d, page size %d, slots %d, rows %d -> %d", pages, blocks, page_size, slots, old_rows, rows);
-  MMAMD_CHECK_ARG((int64_t)slots * page_size <= 1 << 30 && (int64_t)rows + old_rows <= 65535 && (int64_t)rows * slots <= 0x7fffffffll && pages <= 0x7fffffff - 65536 && (int64_t)page_size * row_bytes * blocks <= 0x7fffffffll &&
-                      (int64_t)rows * (((int64_t)page_size * row_bytes * blocks / 16 + 1023) / 1024) <= 0x7fffffffll, MMAMD_E_UNSUPPORTED,
+  MMAMD_CHECK_ARG((int64_t)slots * page_size <= 1 << 30 && (int64_t)rows + old_rows <= 65535 && (int64_t)rows * slots <= 0x7fffffffll && pages <= 0x7fffffff - 65536 && (int64_t)page_size * row_bytes * blocks <= 0x7fffffffll, MMAMD_E_UNSUPPORTED,
                   "mmamd_paged_fork: %d slots of %d tokens, %d rows -> %d", slots, page_size, old_rows, rows);
   MMAMD_CHECK_ARG(pool != nullptr && refcounts != nullptr && new_refcounts != nullptr && shortage != nullptr && workspace != nullptr, MMAMD_E_BADARG, "mmamd_paged_fork: null argument");
   MMAMD_CHECK_ARG((old_rows == 0 || (table != nullptr && lengths != nullptr)) && (rows == 0 || (parents != nullptr && new_table != nullptr && new_lengths != nullptr)), MMAMD_E_BADARG,
@@ -338,17 +379,17 @@ extern "C" int mmamd_paged_fork(void* pool, int pages, int blocks, int page_size
   paged_fork_plan_kernel<<<1 + copiers, 1024, 0, st>>>(p);
   if (int rc = launch_status("paged_fork plan")) return rc;
   if (rows + old_rows == 0) return 0;
-  const uint32_t stretches = (uint32_t)((p.page_bytes / 16 + 1023) / 1024);
-  int64_t grid = (int64_t)rows * stretches;  // no more than 8 workgroups a CU, and one for every four rows
-  if (grid > 2048) grid = 2048;
-  if (grid < (rows + old_rows + 3) / 4) grid = (rows + old_rows + 3) / 4;
-  paged_fork_apply_kernel<<<(unsigned)grid, 256, 0, st>>>(p, stretches, fast_div(stretches));
+  // workgroups of a copy: four pieces a thread if the page is full, but no more than 4096 in all (two rounds of 8 a CU) for many rows
+  int64_t share = (p.page_bytes / 16 + 1023) / 1024;
+  const int64_t most = rows > 0 ? (4096 + rows - 1) / rows : 1;
+  if (share > most) share = most;
+  paged_fork_apply_kernel<<<(unsigned)(rows * share + (rows + old_rows + 3) / 4), 256, 0, st>>>(p, (uint32_t)share, fast_div((uint32_t)share));
   return launch_status("paged_fork");
 }
 
 extern "C" int64_t mmamd_paged_compact_workspace(int pages) {
   MMAMD_CHECK_ARG(pages >= 1, MMAMD_E_BADARG, "mmamd_paged_compact_workspace: pages %d", pages);
-  return 4 * (up4((pages + kCompactPer - 1) / kCompactPer + 1) + 3 * up4(pages));
+  return 4 * (4 + up4((pages + kCompactPer - 1) / kCompactPer) + 3 * up4(pages));
 }
 
 extern "C" int mmamd_paged_compact(void* pool, int pages, int64_t page_bytes, const int32_t* table, int64_t table_row, int rows, int slots, const int32_t* refcounts,
@@ -365,17 +406,23 @@ extern "C" int mmamd_paged_compact(void* pool, int pages, int64_t page_bytes, co
   p.table = table; p.refs = refcounts; p.new_table = new_table; p.new_refs = new_refcounts; p.live = live;
   p.nblk = (pages + kCompactPer - 1) / kCompactPer;
   int32_t* w = reinterpret_cast<int32_t*>(workspace);
-  p.counts = w; w += up4(p.nblk + 1);
+  p.moves = w; w += 4;
+  p.counts = w; w += up4(p.nblk);
   p.rank = w; w += up4(pages);
-  p.src = w; w += up4(pages);
-  p.dst = w;
+  p.moved = reinterpret_cast<int2*>(w);
   p.table_row = table_row; p.page_bytes = page_bytes; p.rows = rows; p.slots = slots; p.pages = pages;
   hipStream_t st = (hipStream_t)stream;
-  paged_compact_count_kernel<<<p.nblk, 1024, 0, st>>>(p);
-  if (int rc = launch_status("paged_compact count")) return rc;
-  paged_compact_plan_kernel<<<p.nblk, 1024, 0, st>>>(p);
+  if (pages <= 16384) {
+    paged_compact_plan_kernel<true><<<p.nblk, 1024, 0, st>>>(p);
+  } else {
+    paged_compact_count_kernel<<<p.nblk, 1024, 0, st>>>(p);
+    if (int rc = launch_status("paged_compact count")) return rc;
+    paged_compact_plan_kernel<false><<<p.nblk, 1024, 0, st>>>(p);
+  }
   if (int rc = launch_status("paged_compact plan")) return rc;
   const uint32_t stretches = (uint32_t)((page_bytes / 16 + 1023) / 1024);
-  paged_compact_apply_kernel<<<2048, 256, 0, st>>>(p, (uint32_t)(page_bytes / 16), stretches, fast_div(stretches));
+  const int64_t entries = (int64_t)rows * slots > pages ? (int64_t)rows * slots : pages;
+  const int64_t copiers = (int64_t)pages * stretches < 2048 ? (int64_t)pages * stretches : 2048, writers = (entries + 255) / 256 < 256 ? (entries + 255) / 256 : 256;
+  paged_compact_apply_kernel<<<(unsigned)(copiers + writers), 256, 0, st>>>(p, (uint32_t)(page_bytes / 16), stretches, fast_div(stretches), (uint32_t)copiers);
   return launch_status("paged_compact");
 }

@@ -275,7 +275,7 @@ def random_tables(g, rows, slots, page, pages, shared):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "fp32"])
-@pytest.mark.parametrize("seed,rows,slots,page,pages", [(0, 1, 1, 1, 4), (1, 4, 5, 16, 40), (2, 9, 7, 5, 200), (3, 33, 4, 8, 150), (4, 6, 3, 16, 5000), (5, 5, 6, 4, 31), (6, 1200, 3, 4, 9000)])
+@pytest.mark.parametrize("seed,rows,slots,page,pages", [(0, 1, 1, 1, 4), (1, 4, 5, 16, 40), (2, 9, 7, 5, 200), (3, 33, 4, 8, 150), (4, 6, 3, 16, 5000), (5, 5, 6, 4, 31), (6, 1200, 3, 4, 9000), (7, 4500, 2, 2, 12000)])
 def test_fork(seed, rows, slots, page, pages, dtype):
     rng = np.random.default_rng(seed)
     table, lengths, refs = random_tables(seed, rows, slots, page, pages, True)
