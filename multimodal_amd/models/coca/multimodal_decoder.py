@@ -73,9 +73,13 @@ class CoCaMultimodalDecoder(nn.Module):
             from ..._autograd import LinearFn  # differentiable vocabulary projection (dgrad + split-K wgrad)
 
             return LinearFn.apply(hidden_states.reshape(B * S, d), self.output_projection.weight, None).unflatten(0, (B, S))
-        h = ops.convert(hidden_states.view(B * S, d), torch.bfloat16)
+        return self.project(hidden_states.view(B * S, d)).unflatten(0, (B, S))
+
+    @torch.jit.unused
+    def project(self, rows: Tensor) -> Tensor:
+        """Vocabulary logits fp32 [n, output_dim] of hidden states fp32 [n, d] (inference)."""
+        h = ops.convert(rows, torch.bfloat16)
         V = self.output_projection.out_features
         w = self._packed.get_padded_rows(self.output_projection.weight, torch.bfloat16, 8)
         out = ops.gemm_bf16(h, w, None, out_dtype=torch.float32)
-        out = out if out.shape[1] == V else out[:, :V]
-        return out.unflatten(0, (B, S))
+        return out if out.shape[1] == V else out[:, :V]

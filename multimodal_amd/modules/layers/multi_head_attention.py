@@ -16,6 +16,7 @@ from ... import _torch_ops, ops
 from ..._autograd import forbid_detached_forward
 from ..._packing import PackedCache
 from ...ops import AttnMask
+from .paged_cache import PagedKVCache
 
 
 _torch_ops.try_load()
@@ -191,6 +192,60 @@ class MultiHeadAttentionWithCache(nn.Module):
         y = ops.gemm_bf16(att, pc.get(self.output_proj.weight, bf), pc.get(self.output_proj.bias, f32), residual=residual,
                           out_dtype=f32, out=out)
         return (y, present) if use_cache else y
+
+    @torch.jit.unused
+    def run_paged(self, x: Tensor, B: int, S: int, cache: PagedKVCache, layer: int, residual: Optional[Tensor], out: Optional[Tensor] = None) -> Tensor:
+        """Self-attention over a cache in pages: x bf16 [B*S, dq] -> fp32 [B*S, dq] = output_proj(attention) (+ residual).  S = 1: each row's new token is stored and
+        attends to all of its row.  S > 1: the prompts of fresh rows (PagedKVCache.add_rows), causal among themselves, are stored."""
+        if self.training and self.dropout > 0:
+            raise ops.MmamdError("this non-differentiable (stand-alone / inference) forward applies no dropout: call .eval()")
+        if B != cache.rows:
+            raise ValueError(f"{B} rows of hidden states for the cache's {cache.rows}")
+        dq, H = self.q_proj.out_features, self.num_heads
+        hd = _check_heads(dq, H)
+        pc, bf, f32 = self._packed, torch.bfloat16, torch.float32
+        w = pc.get_cat([self.q_proj.weight, self.k_proj.weight, self.v_proj.weight], bf)
+        b = pc.get_cat([self.q_proj.bias, self.k_proj.bias, self.v_proj.bias], f32) if self.q_proj.bias is not None else None
+        qkv = ops.gemm_bf16(x, w, b)
+        if S == 1 and cache._prompt is None:
+            q, k, v = qkv.unflatten(1, (3, H, hd)).unbind(1)
+            att = cache.attend(layer, q, k, v).view(B, dq)
+        else:
+            prompt = cache._prompt
+            if prompt is None:
+                raise ops.MmamdError("several tokens a row are stored for fresh rows only (PagedKVCache.add_rows); afterwards one at a time")
+            if isinstance(prompt, int) and prompt != S:
+                raise ValueError(f"add_rows announced prompts of {prompt} tokens, got {S}")
+            k, v = qkv.view(B, S, 3, H, hd)[:, :, 1:].unbind(2)
+            cache.append(layer, k, v, prompt if isinstance(prompt, Tensor) else None)
+            if hd == 64:
+                att = ops.attention_fwd(qkv, B, S, H, causal=True)
+            else:
+                att, _ = ops.attention_x_fwd(qkv[:, :dq], qkv[:, dq:2 * dq], qkv[:, 2 * dq:], B, S, S, H, hd, AttnMask(causal=True))
+        return ops.gemm_bf16(att, pc.get(self.output_proj.weight, bf), pc.get(self.output_proj.bias, f32), residual=residual, out_dtype=f32, out=out)
+
+    @torch.jit.unused
+    def run_paged_cross(self, x: Tensor, cache: PagedKVCache, layer: int, residual: Optional[Tensor], out: Optional[Tensor] = None) -> Tensor:
+        """Cross-attention of one token a row over encoder states whose keys and values are in a cache (store_paged): x bf16 [rows, dq] -> fp32."""
+        if self.training and self.dropout > 0:
+            raise ops.MmamdError("this non-differentiable (stand-alone / inference) forward applies no dropout: call .eval()")
+        dq, H = self.q_proj.out_features, self.num_heads
+        hd = _check_heads(dq, H)
+        pc, bf, f32 = self._packed, torch.bfloat16, torch.float32
+        q = ops.gemm_bf16(x, pc.get(self.q_proj.weight, bf), pc.get(self.q_proj.bias, f32) if self.q_proj.bias is not None else None)
+        att = cache.attend(layer, q.view(-1, H, hd)).view(-1, dq)
+        return ops.gemm_bf16(att, pc.get(self.output_proj.weight, bf), pc.get(self.output_proj.bias, f32), residual=residual, out_dtype=f32, out=out)
+
+    @torch.jit.unused
+    def store_paged(self, states: Tensor, B: int, S: int, cache: PagedKVCache, layer: int) -> None:
+        """Keys and values of encoder states, bf16 [B*S, dim_kv], into a cache (once; every later token reads them)."""
+        dq, H = self.q_proj.out_features, self.num_heads
+        hd = _check_heads(dq, H)
+        pc, bf, f32 = self._packed, torch.bfloat16, torch.float32
+        w = pc.get_cat([self.k_proj.weight, self.v_proj.weight], bf)
+        b = pc.get_cat([self.k_proj.bias, self.v_proj.bias], f32) if self.k_proj.bias is not None else None
+        k, v = ops.gemm_bf16(states, w, b).view(B, S, 2, H, hd).unbind(2)
+        cache.append(layer, k, v)
 
     def forward(self, query: Tensor, key: Tensor, value: Tensor, attn_mask: Optional[Tensor] = None,
                 past_key_value: Optional[Tuple[Tensor, Tensor]] = None, is_causal: bool = False, use_cache: bool = False

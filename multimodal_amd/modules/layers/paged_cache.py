@@ -1,0 +1,115 @@
+"""Key-value cache in pages for serving the decoders (TransformerDecoder, MultiHeadAttentionWithCache): rows (sequences) are continued, forked, dropped and
+added without moving their keys and values, where the reference concatenates the whole cache per token and layer
+(modules/layers/multi_head_attention.py:158-179) and cannot reorder it.  The operators underneath: ops.paged_attention, paged_append, paged_fork, paged_compact."""
+from typing import Optional, Tuple, Union
+
+import torch
+from torch import Tensor
+
+from ... import ops
+
+
+class PagedKVCache:
+    """Keys and values of `n_layer` attention layers for a changing set of rows.
+
+    pages [num_pages, n_layer, 2, num_heads, page_size, head_dim]: a page holds `page_size` tokens of one row for every layer, so that sharing, copying and
+    freeing it is one decision.  page_table int32 [rows, slots], lengths int32 [rows], refcounts int32 [num_pages] as in ops.paged_fork; all on the device, and no
+    method but compact() waits for it.
+
+        cache = PagedKVCache(...)
+        cache.add_rows(batch, prompt_tokens)                # or a tensor of counts
+        decoder(prompt, past_key_values=cache)              # stores the prompt, advances the lengths
+        cache.fork(parents, reserve=1)                      # rows of the next token: beams reordered, rows dropped or doubled
+        decoder(token_states, past_key_values=cache)        # [rows, 1, d]
+
+    num_pages has to cover what is live and, at a fork, what is fresh beside it: rows * (slots + 2) is always enough.  What could not be had is counted in
+    `shortage` (int32 [1], of the last fork); those tokens are lost."""
+
+    def __init__(self, n_layer: int, num_heads: int, head_dim: int, num_pages: int, max_tokens: int, page_size: int = 16, dtype: torch.dtype = torch.bfloat16,
+                 device: Union[str, torch.device] = "cuda") -> None:
+        if head_dim not in (64, 96, 128):
+            raise ops.MmamdError(f"the paged attention kernels are built for 64-, 96- and 128-wide heads, got {head_dim}")
+        if min(n_layer, num_heads, num_pages, max_tokens, page_size) < 1:
+            raise ValueError("n_layer, num_heads, num_pages, max_tokens and page_size must be at least 1")
+        self.page_size, self.max_tokens = page_size, max_tokens
+        self.pages = torch.empty((num_pages, n_layer, 2, num_heads, page_size, head_dim), dtype=dtype, device=device)
+        self.cross: Optional["PagedKVCache"] = None  # keys and values of encoder states, for decoders with cross-attention
+        self.reset()
+
+    def reset(self) -> None:
+        """No rows, every page free."""
+        dev = self.pages.device
+        slots = -(-self.max_tokens // self.page_size)
+        self.page_table = torch.empty((0, slots), dtype=torch.int32, device=dev)
+        self.lengths = torch.empty((0,), dtype=torch.int32, device=dev)
+        self.refcounts = torch.zeros((self.pages.shape[0],), dtype=torch.int32, device=dev)
+        self.shortage = torch.zeros((1,), dtype=torch.int32, device=dev)
+        self._prompt: Union[None, int, Tensor] = None
+
+    @property
+    def rows(self) -> int:
+        return self.page_table.shape[0]
+
+    @property
+    def n_layer(self) -> int:
+        return self.pages.shape[1]
+
+    def layer(self, i: int) -> Tuple[Tensor, Tensor]:
+        """(key_pages, value_pages) of layer i, views [num_pages, num_heads, page_size, head_dim]."""
+        return self.pages[:, i, 0], self.pages[:, i, 1]
+
+    def add_rows(self, rows: int, tokens: Union[int, Tensor]) -> None:
+        """`rows` new rows in the place of the present ones (which must be none, or are dropped), with pages for prompts of `tokens` tokens (an int, or
+        int32 [rows]); the next decoder call stores them."""
+        self.fork(torch.full((rows,), -1, dtype=torch.int32, device=self.pages.device), reserve=tokens)
+        self._prompt = tokens
+
+    def fork(self, parents: Tensor, reserve: Union[int, Tensor] = 1) -> None:
+        """Row r becomes a continuation of the present row parents[r] (int32, any shape, -1: an empty row) with room for `reserve` more tokens."""
+        s = ops.paged_fork(self.pages, self.page_table, self.lengths, self.refcounts, parents.reshape(-1), reserve=reserve)
+        self.page_table, self.lengths, self.refcounts, self.shortage = s
+        self._prompt = None
+
+    def reserve(self, tokens: Union[int, Tensor] = 1) -> None:
+        """Room for `tokens` more tokens in every row."""
+        self.fork(torch.arange(self.rows, dtype=torch.int32, device=self.pages.device), reserve=tokens)
+
+    def shared_rows(self, parents: Tensor) -> "PagedKVCache":
+        """Another view of the same pages: its row r reads what row parents[r] (int64) holds now.  For reading only -- it takes no references, so nothing may be
+        stored, forked or compacted through it, and this cache has to keep the rows."""
+        view = object.__new__(PagedKVCache)
+        view.__dict__.update(self.__dict__)
+        view.page_table, view.lengths = self.page_table[parents], self.lengths[parents]
+        return view
+
+    def append(self, layer: int, k: Tensor, v: Tensor, counts: Optional[Tensor] = None) -> None:
+        """Stores k, v [rows, tokens, num_heads, head_dim] (counts int32 [rows]: the first ones of each row) behind the rows' tokens; advance() is the caller's."""
+        kp, vp = self.layer(layer)
+        ops.paged_append(k, v, kp, vp, self.page_table, self.lengths, counts)
+
+    def attend(self, layer: int, q: Tensor, k: Optional[Tensor] = None, v: Optional[Tensor] = None, scale: Optional[float] = None) -> Tensor:
+        """One token a row: q [rows, heads, head_dim] over the row's tokens in `layer`, and over its new one, which is stored, if k and v are given."""
+        kp, vp = self.layer(layer)
+        return ops.paged_attention(q, kp, vp, self.page_table, self.lengths, k, v, scale)
+
+    def advance(self, tokens: Union[int, Tensor] = 1) -> None:
+        """Counts tokens that every layer has stored."""
+        self.lengths = self.lengths + tokens
+        self._prompt = None
+
+    def compact(self) -> int:
+        """Moves the live pages to the front and says how many they are (this waits for the device)."""
+        self.page_table, self.refcounts, live = ops.paged_compact(self.pages, self.page_table, self.refcounts)
+        return int(live)
+
+    def resize(self, num_pages: int) -> None:
+        """Another number of pages: the live ones are moved to the front and kept, the rest of the memory is given back (or added)."""
+        live = self.compact()
+        if num_pages < max(live, 1):
+            raise ValueError(f"{live} pages are live, {num_pages} are too few")
+        keep = min(num_pages, self.pages.shape[0])
+        pages = torch.empty((num_pages, *self.pages.shape[1:]), dtype=self.pages.dtype, device=self.pages.device)
+        refcounts = torch.zeros((num_pages,), dtype=torch.int32, device=self.pages.device)
+        pages[:live].copy_(self.pages[:live])
+        refcounts[:keep].copy_(self.refcounts[:keep])
+        self.pages, self.refcounts = pages, refcounts

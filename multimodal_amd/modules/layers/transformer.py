@@ -18,6 +18,7 @@ from ..._packing import PackedCache
 from .mlp import MLP
 from .multi_head_attention import MultiHeadAttentionWithCache, MultiHeadSelfAttention, to_attn_mask
 from .normalizations import Fp32LayerNorm
+from .paged_cache import PagedKVCache
 from .stochastic_depth import StochasticDepth
 
 
@@ -319,6 +320,34 @@ class TransformerDecoderLayer(nn.Module):
         y = _ln(pc, self.feedforward_layernorm, ff, f32)
         return (y, present) if caching else y
 
+    @torch.jit.unused
+    def run_paged(self, x: Tensor, B: int, S: int, cache: PagedKVCache, layer: int, enc: Optional[Tensor], Sk: int) -> Tensor:
+        """run() with the self-attention's keys and values in layer `layer` of a paged cache (MultiHeadAttentionWithCache.run_paged).  The cross-attention reads
+        `enc` (bf16 [B*Sk, dim_kv]) where given, else cache.cross."""
+        if self.training and (self.attention_dropout.p > 0 or self.feedforward_dropout.p > 0):
+            raise ops.MmamdError("this non-differentiable forward applies no dropout: call .eval() for inference")
+        bf, f32, pc = torch.bfloat16, torch.float32, self._packed
+        cross = self.use_cross_attention and (enc is not None or cache.cross is not None)
+
+        def cross_attn(h, residual, out):
+            if enc is not None:
+                return self.cross_attention.run(h, enc, B, S, Sk, ops.AttnMask(), residual=residual, out=out)
+            if S != 1:
+                raise ValueError("encoder_hidden_states must be provided for the prompt's cross attention")
+            return self.cross_attention.run_paged_cross(h, cache.cross, layer, residual, out)
+
+        if self.norm_first:
+            a = self.attention.run_paged(_ln(pc, self.attention_layernorm, x, bf), B, S, cache, layer, x)
+            if cross:
+                a = cross_attn(_ln(pc, self.cross_attention_layernorm, a, bf), a, a)
+            return self.feedforward.run(_ln(pc, self.feedforward_layernorm, a, bf), residual=a, out=a)
+        a = _ln(pc, self.attention_layernorm, self.attention.run_paged(ops.convert(x, bf), B, S, cache, layer, x), f32)
+        if self.use_cross_attention:
+            if not cross:
+                raise ValueError("encoder_hidden_states must be provided for cross attention")
+            a = _ln(pc, self.cross_attention_layernorm, cross_attn(ops.convert(a, bf), a, None), f32)
+        return _ln(pc, self.feedforward_layernorm, self.feedforward.run(ops.convert(a, bf), residual=a), f32)
+
     def forward(self, hidden_states: Tensor, encoder_hidden_states: Optional[Tensor] = None, attention_mask: Optional[Tensor] = None,
                 cross_attention_mask: Optional[Tensor] = None, past_key_value: Optional[Tuple[Tensor, Tensor]] = None,
                 use_cache: bool = False) -> Tuple[Tensor, Optional[Tuple[Tensor, Tensor]]]:
@@ -452,6 +481,10 @@ class TransformerDecoder(nn.Module):
                       cross_attention_mask: Optional[Tensor] = None, past_key_values: Optional[List[Tuple[Tensor, Tensor]]] = None,
                       use_cache: bool = False, return_hidden_states: bool = False) -> TransformerOutput:
         B, S, d = hidden_states.shape
+        if isinstance(past_key_values, PagedKVCache):
+            if attention_mask is not None:
+                raise ops.MmamdError("with a paged cache the self-attention is causal over each row's tokens: no attention_mask")
+            return self._forward_paged(hidden_states, encoder_hidden_states, past_key_values, return_hidden_states)
         caching = past_key_values is not None or use_cache
         if not plain_layers(self.layer, TransformerDecoderLayer):
             # the reference's own loop (:606-640), every layer CALLED as a module (wrapped / hooked layers)
@@ -501,6 +534,63 @@ class TransformerDecoder(nn.Module):
         if self.final_layer_norm is not None:
             x = self.final_layer_norm(x)
         return TransformerOutput(last_hidden_state=x, hidden_states=all_hidden_states, current_key_values=current_key_values)
+
+
+def _decoder_forward_paged(self, hidden_states: Tensor, encoder_hidden_states, cache: PagedKVCache, return_hidden_states: bool) -> TransformerOutput:
+    """Incremental decoding with the keys and values in pages: hidden_states [rows, 1, d] are the rows' next tokens, or [rows, tokens, d] their prompts (after
+    PagedKVCache.add_rows).  Every layer stores them, then the cache's lengths are advanced; current_key_values is the cache."""
+    if wants_grad(self) or (torch.is_grad_enabled() and hidden_states.requires_grad):
+        raise ops.MmamdError("key/value caching is an inference feature: call the decoder under torch.no_grad() / in eval mode")
+    if not plain_layers(self.layer, TransformerDecoderLayer):
+        raise ops.MmamdError("a paged cache is served by the decoder's own layers only (not wrapped or hooked ones)")
+    if cache.n_layer != len(self.layer):
+        raise ValueError(f"the cache has {cache.n_layer} layers, the decoder {len(self.layer)}")
+    B, S, d = hidden_states.shape
+    x = _f32_rows(hidden_states, "TransformerDecoder")
+    enc, Sk = None, 0
+    if encoder_hidden_states is not None:
+        Sk = encoder_hidden_states.shape[1]
+        enc = ops.convert(_f32_rows(encoder_hidden_states, "TransformerDecoder"), torch.bfloat16)
+    hidden = []
+    prompt = cache._prompt
+    for i, layer_module in enumerate(self.layer):
+        if return_hidden_states:
+            hidden.append(x.view(B, S, d))
+        x = layer_module.run_paged(x, B, S, cache, i, enc, Sk)
+    cache.advance(1 if prompt is None else prompt)
+    x = x.view(B, S, d)
+    if return_hidden_states:
+        hidden.append(x)
+    if self.final_layer_norm is not None:
+        x = self.final_layer_norm(x)
+    return TransformerOutput(last_hidden_state=x, hidden_states=hidden, current_key_values=cache)
+
+
+TransformerDecoder._forward_paged = _decoder_forward_paged
+
+
+def _decoder_cross_cache(self, encoder_hidden_states: Tensor, page_size: int = 16) -> PagedKVCache:
+    """Keys and values of encoder states [rows, tokens, dim_kv] for every layer's cross-attention, in a cache of their own: assign it (or its
+    shared_rows) to the `cross` of the self-attention's cache, row for row."""
+    if wants_grad(self) or (torch.is_grad_enabled() and encoder_hidden_states.requires_grad):
+        raise ops.MmamdError("key/value caching is an inference feature: call it under torch.no_grad() / in eval mode")
+    B, Sk, _ = encoder_hidden_states.shape
+    enc = ops.convert(_f32_rows(encoder_hidden_states, "TransformerDecoder"), torch.bfloat16)
+    att = next((m.cross_attention for m in self.layer if m.cross_attention is not None), None)
+    if att is None:
+        raise ValueError("the decoder has no cross-attention")
+    slots = -(-Sk // page_size)
+    cache = PagedKVCache(len(self.layer), att.num_heads, att.q_proj.out_features // att.num_heads, max(1, B * slots), max(1, Sk), page_size,
+                         device=encoder_hidden_states.device)
+    cache.add_rows(B, Sk)
+    for i, layer_module in enumerate(self.layer):
+        if layer_module.cross_attention is not None:
+            layer_module.cross_attention.store_paged(enc, B, Sk, cache, i)
+    cache.advance(Sk)
+    return cache
+
+
+TransformerDecoder.cross_cache = _decoder_cross_cache
 
 
 def _decoder_forward_train(self, hidden_states: Tensor, encoder_hidden_states, attention_mask, return_hidden_states: bool) -> TransformerOutput:

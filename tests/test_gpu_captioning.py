@@ -1,0 +1,172 @@
+"""The decoding operators in the models: TransformerDecoder over a paged cache against the reference's fixture and its own full pass, and captions of a CoCa model
+against full forwards."""
+import numpy as np
+import pytest
+import torch
+
+from tests.golden.make_golden import seed
+from tests.golden.make_golden_coca import POOL96, SMALL, randomize
+
+pytestmark = pytest.mark.gpu
+
+LOGIT_TOL = 3e-2  # of the vocabulary logits, as in test_gpu_coca.py
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _built():
+    from multimodal_amd import build
+
+    build.build()
+
+
+def host(t):
+    return t.detach().float().cpu().numpy().astype(np.float64)
+
+
+def cache_for(dec, rows, max_tokens, page_size):
+    from multimodal_amd.modules.layers.paged_cache import PagedKVCache
+
+    att = dec.layer[0].attention
+    slots = -(-max_tokens // page_size)
+    return PagedKVCache(len(dec.layer), att.num_heads, att.q_proj.out_features // att.num_heads, rows * (slots + 2), max_tokens, page_size)
+
+
+@pytest.mark.parametrize("page_size", [1, 4, 16])
+@pytest.mark.parametrize("cross_cached", [False, True])
+@torch.no_grad()
+def test_decoder_over_a_paged_cache_vs_reference_fixture(golden, page_size, cross_cached):
+    """A prompt and two single tokens through pages equal the reference's causal pass, as the concatenated cache does (tests/test_gpu_coca.py)."""
+    from multimodal_amd.modules.layers.transformer import TransformerDecoder
+
+    z = golden("kv_cache.npz")
+    dec = TransformerDecoder(n_layer=2, d_model=128, n_head=2, dim_feedforward=256, activation=torch.nn.GELU, layer_norm_eps=1e-5, norm_first=True,
+                             use_cross_attention=True, dim_kv=128, final_layer_norm_eps=1e-5)
+    dec.load_state_dict({k[7:]: torch.from_numpy(z[k]) for k in z.files if k.startswith("dec.sd.")}, strict=True)
+    dec = dec.cuda().eval()
+    h, enc = torch.from_numpy(z["dec.h"]).cuda(), torch.from_numpy(z["dec.enc"]).cuda()
+    full = dec(h, enc, attention_mask=torch.ones(6, 6, dtype=torch.bool).tril().cuda()).last_hidden_state
+    cache = cache_for(dec, 2, 6, page_size)
+    if cross_cached:
+        cache.cross = dec.cross_cache(enc, page_size)
+    cache.add_rows(2, 4)
+    o = dec(h[:, :4], enc, past_key_values=cache, return_hidden_states=True)
+    assert o.current_key_values is cache and len(o.hidden_states) == 3 and host(cache.lengths).tolist() == [4, 4]
+    steps = [o.last_hidden_state]
+    for t in (4, 5):
+        cache.reserve(1)
+        steps.append(dec(h[:, t:t + 1], None if cross_cached else enc, past_key_values=cache).last_hidden_state)
+    inc = torch.cat(steps, dim=1)
+    assert np.abs(host(inc) - z["dec.full"]).max() <= 4e-2
+    assert np.abs(host(inc) - host(full)).max() <= 2e-2
+    assert int(cache.shortage) == 0
+    with pytest.raises(ValueError):
+        dec(h[:1, :1], enc, past_key_values=cache)
+    with pytest.raises(RuntimeError):
+        dec(h[:, :2], enc, past_key_values=cache)  # several tokens behind others
+    with pytest.raises(RuntimeError):
+        dec(h[:, :1], enc, attention_mask=torch.ones(1, 1, dtype=torch.bool).cuda(), past_key_values=cache)
+
+
+@torch.no_grad()
+def test_decoder_ragged_prompts_forks_and_resize():
+    """Prompts of different lengths (padded), one longer than the concatenated cache's attention takes; rows forked and dropped; the pool cut down on the way:
+    every row equals the causal pass over its own tokens."""
+    from multimodal_amd.modules.layers.transformer import TransformerDecoder
+
+    torch.manual_seed(0)
+    dec = TransformerDecoder(n_layer=2, d_model=192, n_head=3, dim_feedforward=256, activation=torch.nn.GELU, layer_norm_eps=1e-5, norm_first=False,
+                             use_cross_attention=False).cuda().eval()
+    g = torch.Generator().manual_seed(1)
+    counts = [300, 1, 17]
+    rows = [torch.randn(n, 192, generator=g) for n in counts]
+    cache = cache_for(dec, 6, 400, 16)
+    cache.add_rows(3, torch.tensor(counts, dtype=torch.int32, device="cuda"))
+    prompt = torch.nn.utils.rnn.pad_sequence(rows, batch_first=True)
+    out = dec(prompt.cuda(), past_key_values=cache).last_hidden_state
+    assert host(cache.lengths).tolist() == counts
+    got = [out[r, n - 1] for r, n in enumerate(counts)]
+    for step, parents in enumerate([[0, 0, 1, 2], [3, 2, 1, 1, 0], [4, 0, 2]]):
+        cache.fork(torch.tensor(parents, dtype=torch.int32, device="cuda"), reserve=1)
+        if step == 1:
+            cache.resize(60)
+        new = torch.randn(len(parents), 1, 192, generator=g)
+        rows = [torch.cat([rows[p], x]) for p, x in zip(parents, new)]
+        got = dec(new.cuda(), past_key_values=cache).last_hidden_state[:, 0]
+        assert int(cache.shortage) == 0
+    for r, row in enumerate(rows):
+        full = dec(row[None].cuda(), attention_mask=None if len(row) == 1 else causal(len(row))).last_hidden_state[0, -1] if len(row) <= 288 else None
+        if full is not None:
+            assert np.abs(host(got[r]) - host(full)).max() <= 2e-2
+    assert any(len(row) > 288 for row in rows)
+    # the long row: its last state again from a prompt of all its tokens
+    long = max(rows, key=len)
+    again = cache_for(dec, 1, 400, 7)
+    again.add_rows(1, len(long))
+    want = dec(long[None].cuda(), past_key_values=again).last_hidden_state[0, -1]
+    assert np.abs(host(got[[len(r) for r in rows].index(len(long))]) - host(want)).max() <= 2e-2
+    with pytest.raises(ValueError):
+        cache.resize(3)
+
+
+def causal(n):
+    return torch.ones(n, n, dtype=torch.bool, device="cuda").tril()
+
+
+def coca(cfg, cascaded, seed_v):
+    from multimodal_amd.models.coca.coca_model import coca_vit
+
+    seed(seed_v)
+    model = coca_vit(**cfg, cascaded_pooler=cascaded).eval()
+    randomize(model, torch.Generator().manual_seed(seed_v + 1))
+    with torch.no_grad():
+        model.multimodal_decoder.output_projection.weight.mul_(6.0)  # spread the words, so that rounding rarely decides
+    return model.cuda()
+
+
+def full_log_probs(model, images, sequences):
+    """log p(next word) [n, tokens, vocab] in 64 bits from the model's own full forward over the sequences [n, tokens]."""
+    ids = sequences.clone()
+    pad = model.text_decoder.num_positions - 1 - ids.shape[1]
+    ids = torch.nn.functional.pad(ids, (0, pad), value=0)
+    return torch.log_softmax(model(images, ids).multimodal_embeddings.double(), -1)[:, :sequences.shape[1]]
+
+
+@pytest.mark.parametrize("cfg,cascaded", [(SMALL, False), (SMALL, True), (POOL96, False)], ids=["parallel", "cascaded", "three-heads"])
+@torch.no_grad()
+def test_captions_vs_full_forward(cfg, cascaded):
+    from multimodal_amd.models.coca.captioning import generate_captions
+
+    model = coca(cfg, cascaded, 61)
+    images = torch.randn(3, 3, 64, 64, generator=torch.Generator().manual_seed(5)).cuda()
+    end = 2
+    greedy = generate_captions(model, images, 1, end, num_beams=1, length_penalty=0.0)
+    assert greedy.sequences.shape == (3, 1, 12) and (greedy.sequences[:, :, 0] == 1).all()
+    logp = full_log_probs(model, images, greedy.sequences[:, 0])
+    for b in range(3):
+        total = 0.0
+        for t in range(int(greedy.lengths[b, 0])):
+            word = int(greedy.sequences[b, 0, t + 1])
+            assert float(logp[b, t].max() - logp[b, t, word]) <= 2 * LOGIT_TOL * 6  # the best word, or one that rounding cannot tell from it
+            total += float(logp[b, t, word])
+        assert abs(total - float(greedy.scores[b, 0])) <= 2 * LOGIT_TOL * 6 * int(greedy.lengths[b, 0])
+    for penalty, page in ((0.0, 16), (1.0, 4)):
+        beams = generate_captions(model, images, 1, end, num_beams=4, length_penalty=penalty, page_size=page)
+        rank = host(beams.scores) / np.maximum(host(beams.lengths), 1) ** penalty
+        assert (np.diff(rank, axis=1) <= 1e-6).all()  # best first
+        for k in range(4):
+            logp = full_log_probs(model, images, beams.sequences[:, k])
+            for b in range(3):
+                n = int(beams.lengths[b, k])
+                words = beams.sequences[b, k, 1:]
+                total = sum(float(logp[b, t, int(words[t])]) for t in range(n))
+                assert abs(total - float(beams.scores[b, k])) <= 2 * LOGIT_TOL * 6 * n
+                assert (words[:n - 1] != end).all() and (n == 11 or int(words[n - 1]) == end) and (words[n:] == end).all()
+            for j in range(k):
+                assert not (beams.sequences[:, k] == beams.sequences[:, j]).all(-1).any()  # the beams of an image differ
+    again = generate_captions(model, images, 1, end, num_beams=4, length_penalty=1.0, page_size=4)
+    assert torch.equal(again.sequences, beams.sequences) and torch.equal(again.scores, beams.scores)
+    short = generate_captions(model, images[:1], 1, end, num_beams=2, max_length=3)
+    assert short.sequences.shape == (1, 2, 3)
+    model.train()
+    with pytest.raises(RuntimeError):
+        generate_captions(model, images, 1, end)

@@ -197,3 +197,29 @@ def test_oracle_beam_equals_sort():
         np.testing.assert_allclose(res[0][g], flat[best])
         np.testing.assert_array_equal(res[3][g], best % 11)
         np.testing.assert_array_equal(res[4][g], best // 11 + 3 * g)
+
+
+def test_cache_and_captioning_arguments():
+    from multimodal_amd import ops
+    from multimodal_amd.models.coca.captioning import generate_captions
+    from multimodal_amd.models.coca.coca_model import coca_vit
+    from multimodal_amd.modules.layers.paged_cache import PagedKVCache
+    from tests.golden.make_golden_coca import SMALL
+
+    with pytest.raises(ops.MmamdError, match="wide heads"):
+        PagedKVCache(1, 2, 80, 4, 16, device="cpu")
+    with pytest.raises(ValueError):
+        PagedKVCache(1, 2, 64, 0, 16, device="cpu")
+    cache = PagedKVCache(2, 3, 64, 5, 33, 16, device="cpu")
+    assert cache.pages.shape == (5, 2, 2, 3, 16, 64) and cache.page_table.shape == (0, 3) and cache.rows == 0
+    assert cache.layer(1)[0].data_ptr() == cache.pages[0, 1, 0].data_ptr()
+    with pytest.raises(ops.MmamdError, match="no CPU fallback"):
+        cache.add_rows(2, 1)
+    model = coca_vit(**SMALL, cascaded_pooler=False)
+    images = torch.zeros(1, 3, 64, 64)
+    with pytest.raises(ops.MmamdError, match="eval"):
+        generate_captions(model, images, 1, 2)
+    model.eval()
+    for kw in (dict(max_length=1), dict(max_length=13), dict(num_beams=0)):
+        with pytest.raises(ValueError):
+            generate_captions(model, images, 1, 2, **kw)
