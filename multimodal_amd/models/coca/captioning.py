@@ -27,11 +27,79 @@ def captioning_embeddings(model: CoCaModel, images: Tensor) -> Tensor:
     return pooled[0] if isinstance(pooled, list) else pooled[:, 1:]
 
 
+class _Search:
+    """The state of one search in tensors that stay where they are, so that a step can be captured in a HIP graph and replayed."""
+
+    def __init__(self, model: CoCaModel, states: Tensor, begin: int, end: int, beams: int, max_length: int, length_penalty: float, page_size: int) -> None:
+        self.text, self.fusion, self.end, self.length_penalty = model.text_decoder.transformer_decoder, model.multimodal_decoder, end, length_penalty
+        emb = model.text_decoder.embeddings
+        self.table = emb._packed.get(emb.token_embeddings.weight, torch.float32)
+        self.positions = emb._packed.get(emb.position_embeddings, torch.float32)
+        bsz, dev = states.shape[0], states.device
+        rows = self.rows = bsz * beams
+        self.caches = []
+        for decoder in (self.text, self.fusion.transformer_decoder):
+            att = decoder.layer[0].attention
+            pages = rows * (-(-max_length // page_size) + 2)
+            self.caches.append(PagedKVCache(len(decoder.layer), att.num_heads, att.q_proj.out_features // att.num_heads, max(1, pages), max_length, page_size, device=dev))
+        # the beams of an image read the same pages, and a beam is only ever continued within its image: one table for the whole search
+        cross = self.fusion.transformer_decoder.cross_cache(states.contiguous(), page_size)
+        self.caches[1].cross = cross.shared_rows(torch.arange(bsz, device=dev).repeat_interleave(beams))
+        for cache in self.caches:
+            cache.fork(torch.full((rows,), -1, dtype=torch.int32, device=dev), reserve=1)
+        self.scores = torch.full((bsz, beams), float("-inf"), device=dev)
+        self.scores[:, 0] = 0.0
+        self.lengths = torch.zeros((bsz, beams), dtype=torch.int32, device=dev)
+        self.finished = torch.zeros((bsz, beams), dtype=torch.bool, device=dev)
+        self.sequences = torch.full((bsz, beams, max_length - 1), end, dtype=torch.int64, device=dev)  # what follows the begin token
+        self.tokens = torch.full((bsz, beams), begin, dtype=torch.int64, device=dev)
+        self.place = self.positions[:1].clone()
+        self.held = [[c.page_table, c.lengths, c.refcounts] for c in self.caches]
+
+    def step(self) -> None:
+        """One more token of every beam."""
+        x = ops.embed_tokens(self.tokens.view(self.rows, 1), self.table, self.place).view(self.rows, 1, -1)
+        x = self.text(x, past_key_values=self.caches[0]).last_hidden_state
+        x = self.fusion.transformer_decoder(x, past_key_values=self.caches[1]).last_hidden_state
+        r = ops.beam_search_step(self.fusion.project(x.view(self.rows, -1)), self.scores, self.lengths, self.finished, self.sequences, self.end, self.length_penalty)
+        for to, new in zip((self.scores, self.lengths, self.finished, self.tokens, self.sequences), (r.scores, r.lengths, r.finished, r.tokens, r.sequences)):
+            to.copy_(new)
+        for cache, held in zip(self.caches, self.held):
+            cache.fork(r.parents, reserve=1)
+            for to, new in zip(held, (cache.page_table, cache.lengths, cache.refcounts)):
+                to.copy_(new)
+            cache.page_table, cache.lengths, cache.refcounts = held
+
+    def run(self, steps: int, graph: bool) -> None:
+        replay = None
+        for t in range(steps):
+            self.place.copy_(self.positions[t:t + 1])
+            if graph and replay is None and t == 2 and steps > 4:
+                # two steps went before on this stream, with a wait between them: the kernel-ready weights are made and nobody waits for their making
+                replay = torch.cuda.CUDAGraph()
+                replay.capture_begin()
+                try:
+                    self.step()
+                finally:
+                    replay.capture_end()
+            if replay is None:
+                self.step()
+                if t == 0 and graph:
+                    torch.cuda.current_stream().synchronize()
+            else:
+                replay.replay()
+            if t % 8 == 7 and bool(self.finished.all()):
+                break
+        if replay is not None:
+            torch.cuda.current_stream().synchronize()  # the graph's own memory goes with it
+
+
 @torch.no_grad()
 def generate_captions(model: CoCaModel, images: Tensor, begin: int, end: int, num_beams: int = 5, max_length: Optional[int] = None,
-                      length_penalty: float = 1.0, page_size: int = 16) -> Captions:
+                      length_penalty: float = 1.0, page_size: int = 16, graph: bool = True) -> Captions:
     """Captions of images [bsz, ...] by beam search from token `begin` until every beam has taken `end` or has max_length tokens (default and at most: the
-    text decoder's positions without its CLS).  Ranked by log-probability / length ** length_penalty."""
+    text decoder's positions without its CLS).  Ranked by log-probability / length ** length_penalty.  graph: from the third token on a step is a replayed
+    HIP graph, in place of some three hundred launches from Python."""
     if model.training:
         raise ops.MmamdError("generate_captions: call model.eval() first")
     text, fusion = model.text_decoder, model.multimodal_decoder
@@ -43,44 +111,22 @@ def generate_captions(model: CoCaModel, images: Tensor, begin: int, end: int, nu
         raise ValueError(f"num_beams must be at least 1, got {num_beams}")
     if fusion.output_projection is None:
         raise ValueError("the multimodal decoder has no output projection to the vocabulary")
-    emb = text.embeddings
-    table, positions = emb._packed.get(emb.token_embeddings.weight, torch.float32), emb._packed.get(emb.position_embeddings, torch.float32)
+    vocab = text.embeddings.token_embeddings.num_embeddings
+    if not (0 <= begin < vocab and 0 <= end < min(vocab, fusion.output_projection.out_features)) or fusion.output_projection.out_features > vocab:
+        raise ValueError(f"begin {begin} and end {end} must be words of the vocabulary of {vocab}, which the output projection must not exceed")
+    if images.shape[0] == 0:  # (the encoders take no empty batch)
+        empty = torch.zeros((0, num_beams), device=images.device)
+        return Captions(empty[:, :, None].expand(0, num_beams, max_length).long(), empty, empty.int())
     states = captioning_embeddings(model, images)
-    bsz, dev = states.shape[0], states.device
-    rows = bsz * num_beams
-
-    def cache_of(decoder) -> PagedKVCache:
-        att = decoder.layer[0].attention
-        slots = -(-max_length // page_size)
-        return PagedKVCache(len(decoder.layer), att.num_heads, att.q_proj.out_features // att.num_heads, max(1, rows * (slots + 2)), max_length, page_size, device=dev)
-
-    caches = [cache_of(text.transformer_decoder), cache_of(fusion.transformer_decoder)]
-    # the beams of an image read the same pages, and a beam is only ever continued within its image: one table for the whole search
-    cross = fusion.transformer_decoder.cross_cache(states.contiguous(), page_size)
-    caches[1].cross = cross.shared_rows(torch.arange(bsz, device=dev).repeat_interleave(num_beams))
-    for cache in caches:
-        cache.add_rows(rows, 1)
-        cache._prompt = None  # the first token is a step like the others
-
-    scores = torch.full((bsz, num_beams), float("-inf"), device=dev)
-    scores[:, 0] = 0.0
-    lengths = torch.zeros((bsz, num_beams), dtype=torch.int32, device=dev)
-    finished = torch.zeros((bsz, num_beams), dtype=torch.bool, device=dev)
-    sequences = torch.full((bsz, num_beams, max_length), end, dtype=torch.int64, device=dev)
-    sequences[:, :, 0] = begin
-    tokens = sequences[:, :, 0].contiguous()
-    if rows == 0:
-        return Captions(sequences, scores, lengths)
-    for t in range(max_length - 1):
-        x = ops.embed_tokens(tokens.view(rows, 1), table, positions[t:t + 1].contiguous()).view(rows, 1, -1)
-        x = text.transformer_decoder(x, past_key_values=caches[0]).last_hidden_state
-        x = fusion.transformer_decoder(x, past_key_values=caches[1]).last_hidden_state
-        # what follows the begin token is chosen and reordered; it is the same for every beam
-        step = ops.beam_search_step(fusion.project(x.view(rows, -1)), scores, lengths, finished, sequences[:, :, 1:].contiguous(), end, length_penalty)
-        scores, lengths, finished, tokens = step.scores, step.lengths, step.finished, step.tokens
-        sequences = torch.cat([sequences[:, :, :1], step.sequences], dim=2)  # (data movement)
-        if t + 2 >= max_length or (t % 8 == 7 and bool(finished.all())):
-            break
-        for cache in caches:
-            cache.fork(step.parents, reserve=1)
-    return Captions(sequences, scores, lengths)
+    main = torch.cuda.current_stream()
+    side = torch.cuda.Stream() if graph else main  # (the legacy default stream cannot be captured)
+    side.wait_stream(main)
+    with torch.cuda.stream(side):
+        search = _Search(model, states, begin, end, num_beams, max_length, length_penalty, page_size)
+        search.run(max_length - 1, graph)
+        first = torch.full((states.shape[0], num_beams, 1), begin, dtype=torch.int64, device=states.device)
+        result = Captions(torch.cat([first, search.sequences], dim=2), search.scores, search.lengths)
+    main.wait_stream(side)
+    for t in (*result, states):
+        t.record_stream(main)
+    return result

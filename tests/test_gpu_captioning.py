@@ -165,6 +165,10 @@ def test_captions_vs_full_forward(cfg, cascaded):
                 assert not (beams.sequences[:, k] == beams.sequences[:, j]).all(-1).any()  # the beams of an image differ
     again = generate_captions(model, images, 1, end, num_beams=4, length_penalty=1.0, page_size=4)
     assert torch.equal(again.sequences, beams.sequences) and torch.equal(again.scores, beams.scores)
+    eager = generate_captions(model, images, 1, end, num_beams=4, length_penalty=1.0, page_size=4, graph=False)  # replays equal eager steps, bit for bit
+    assert torch.equal(eager.sequences, beams.sequences) and torch.equal(eager.scores, beams.scores) and torch.equal(eager.lengths, beams.lengths)
+    none = generate_captions(model, images[:0], 1, end, num_beams=2)
+    assert none.sequences.shape == (0, 2, 12) and none.scores.shape == (0, 2)
     short = generate_captions(model, images[:1], 1, end, num_beams=2, max_length=3)
     assert short.sequences.shape == (1, 2, 3)
     model.train()

@@ -220,6 +220,6 @@ def test_cache_and_captioning_arguments():
     with pytest.raises(ops.MmamdError, match="eval"):
         generate_captions(model, images, 1, 2)
     model.eval()
-    for kw in (dict(max_length=1), dict(max_length=13), dict(num_beams=0)):
+    for kw in (dict(max_length=1), dict(max_length=13), dict(num_beams=0), dict(begin=96), dict(end=-1)):
         with pytest.raises(ValueError):
-            generate_captions(model, images, 1, 2, **kw)
+            generate_captions(model, images, **{"begin": 1, "end": 2, **kw})
