@@ -68,7 +68,17 @@ __device__ __forceinline__ uint4 load_piece(const char* at) {
 //   out [dim, head] += V^T . weights: the values go through LDS for their columns, the weights are where the first product left them.
 // A pass over a tile ends with the loads of the next one in flight, and the page numbers of the one after.  fp32 runs on the fp32 matrix instruction.
 // bf16 weights are split in two bf16 parts (2^-16 of a weight is lost): in one part they would lose as much as the output's own rounding.
-template <typename T, int D, bool STREAM>
+// the maximum over the four lanes l, l + 16, l + 32, l + 48, in each of them (a shuffle would go through LDS)
+__device__ __forceinline__ float across_quarters_max(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// GROUPS: 16 tokens that begin at a multiple of 16 lie in one page (the page size is a multiple of 16), so their addresses are one scalar and a
+// constant lane offset; otherwise every lane finds the page of one token and the others' come by shuffles.
+template <typename T, int D, bool STREAM, bool GROUPS>
 __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const PagedAttnParams p) {
   constexpr int TOK = sizeof(T) == 2 ? 32 : 16;      // tokens of a tile
   constexpr int NT = TOK / 16;
@@ -104,32 +114,89 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const PagedAttnParam
   const char* const knew = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.k) + row * p.k_row + kvh * p.k_head);
   const char* const vnew = reinterpret_cast<const char*>(reinterpret_cast<const T*>(p.v) + row * p.v_row + kvh * p.v_head);
 
+  constexpr int VG = VP / NT;                        // pieces of values per lane and 16 tokens
   uint4 kr[NT][KP], vr[VP];
   uint32_t okmask = 0;                               // which tokens of the loaded tile take part
-  auto page_of = [&](int t0) {                       // page number of token t0 + lane % TOK; -1 behind the split's end
-    const int t = t0 + (lane & (TOK - 1));
-    const int id = t < end ? table[div_by(p.page, (uint32_t)t)] : -1;
-    return (uint32_t)id < (uint32_t)p.pages ? id : -1;
+  constexpr uint32_t ALL = TOK == 32 ? 0xffffffffu : 0xffffu;
+  auto value_place = [&](int i, int& tok, int& x) {  // piece i of this lane: its token in the tile, its place in the token's row
+    const int piece = i % VG * 64 + lane;
+    tok = i / VG * 16 + piece / PIECES;
+    x = piece % PIECES;
   };
-  auto load_tile = [&](int t0, int id) {
-    const int t = t0 + (lane & (TOK - 1));
-    okmask = (uint32_t)__ballot(id >= 0 && lane < TOK);
-    const int off = t - (int)(div_by(p.page, (uint32_t)t) * p.page.d);
-    const int64_t pg = id >= 0 ? id : 0;             // a place that holds no token is read as page 0, which exists, and not used
-    int64_t ko = (pg * p.key_page + off * p.key_token) * (int64_t)sizeof(T), vo = (pg * p.value_page + off * p.value_token) * (int64_t)sizeof(T);
-    if (id >= 0 && t == pos) { ko = knew - keys; vo = vnew - values; }
-    const int klo = (int)ko, khi = (int)(ko >> 32), vlo = (int)vo, vhi = (int)(vo >> 32);
+  // The tile's page numbers, raw: looking at one here would wait for it and thereby for the tile that was just requested.  For groups they are scalar loads,
+  // which count apart from the others (the table is not written while this runs: the address space says so).
+  struct Ids { int id[GROUPS ? NT : 1]; };
+  typedef const __attribute__((address_space(4))) int32_t* const_ptr;
+  auto page_of = [&](int t0) {
+    Ids r;
+    if constexpr (GROUPS) {
 #pragma unroll
-    for (int u = 0; u < NT; ++u) {
-      const int64_t o = (int64_t)(((uint64_t)(uint32_t)__shfl(khi, u * 16 + l15) << 32) | (uint32_t)__shfl(klo, u * 16 + l15));
-#pragma unroll
-      for (int i = 0; i < KP; ++i) kr[u][i] = load_piece<STREAM>(keys + o + (i * 4 + quarter) * 16);
+      for (int u = 0; u < NT; ++u) {
+        const int t = t0 + u * 16;
+        r.id[u] = ((const_ptr)(uintptr_t)table)[div_by(p.page, (uint32_t)(t < end ? t : end - 1))];
+      }
+    } else {
+      const int t = t0 + (lane & (TOK - 1));
+      r.id[0] = table[div_by(p.page, (uint32_t)(t < end ? t : end - 1))];
     }
+    return r;
+  };
+  const uint32_t klane = (uint32_t)(l15 * p.key_token * (int64_t)sizeof(T)) + quarter * 16;  // (GROUPS only, where it fits)
+  auto load_tile = [&](int t0, const Ids& ids) {
+    if constexpr (GROUPS) {
+      okmask = 0;
 #pragma unroll
-    for (int i = 0; i < VP; ++i) {
-      const int piece = i * 64 + lane, tok = piece / PIECES, x = piece - tok * PIECES;
-      const int64_t o = (int64_t)(((uint64_t)(uint32_t)__shfl(vhi, tok) << 32) | (uint32_t)__shfl(vlo, tok));
-      vr[i] = load_piece<STREAM>(values + o + x * 16);
+      for (int u = 0; u < NT; ++u) {
+        const int t = t0 + u * 16, off = t - (int)(div_by(p.page, (uint32_t)t) * p.page.d), left = end - t;
+        const bool inside = (uint32_t)ids.id[u] < (uint32_t)p.pages && left > 0;
+        if (inside) okmask |= (left >= 16 ? 0xffffu : (1u << left) - 1u) << (u * 16);
+        const int64_t pg = inside ? ids.id[u] : 0;           // a place that holds no token is read as page 0, which exists, and not used
+        const char* kb = keys + (pg * p.key_page + off * p.key_token) * (int64_t)sizeof(T);
+        const char* vb = values + (pg * p.value_page + off * p.value_token) * (int64_t)sizeof(T);
+#pragma unroll
+        for (int i = 0; i < KP; ++i) kr[u][i] = load_piece<STREAM>(kb + klane + i * 64);
+#pragma unroll
+        for (int i = 0; i < VG; ++i) {
+          int tok, x;
+          value_place(i, tok, x);
+          vr[u * VG + i] = load_piece<STREAM>(vb + (uint32_t)(tok * p.value_token * (int64_t)sizeof(T)) + x * 16);
+        }
+      }
+    } else {
+      const int t = t0 + (lane & (TOK - 1)), id = ids.id[0];
+      const bool inside = (uint32_t)id < (uint32_t)p.pages && t < end;
+      okmask = (uint32_t)__ballot(inside && lane < TOK);
+      const int off = t - (int)(div_by(p.page, (uint32_t)t) * p.page.d);
+      const int64_t pg = inside ? id : 0;
+      const int64_t ko = (pg * p.key_page + off * p.key_token) * (int64_t)sizeof(T), vo = (pg * p.value_page + off * p.value_token) * (int64_t)sizeof(T);
+      const int klo = (int)ko, khi = (int)(ko >> 32), vlo = (int)vo, vhi = (int)(vo >> 32);
+#pragma unroll
+      for (int u = 0; u < NT; ++u) {
+        const int64_t o = (int64_t)(((uint64_t)(uint32_t)__shfl(khi, u * 16 + l15) << 32) | (uint32_t)__shfl(klo, u * 16 + l15));
+#pragma unroll
+        for (int i = 0; i < KP; ++i) kr[u][i] = load_piece<STREAM>(keys + o + (i * 4 + quarter) * 16);
+      }
+#pragma unroll
+      for (int i = 0; i < VP; ++i) {
+        int tok, x;
+        value_place(i, tok, x);
+        const int64_t o = (int64_t)(((uint64_t)(uint32_t)__shfl(vhi, tok) << 32) | (uint32_t)__shfl(vlo, tok));
+        vr[i] = load_piece<STREAM>(values + o + x * 16);
+      }
+    }
+    if (pos >= t0 && pos < t0 + TOK && (okmask >> (pos - t0) & 1u)) {  // the new token is not in its place yet
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+        if (t0 + u * 16 + l15 == pos) {
+#pragma unroll
+          for (int i = 0; i < KP; ++i) kr[u][i] = *reinterpret_cast<const uint4*>(knew + (i * 4 + quarter) * 16);
+        }
+#pragma unroll
+      for (int i = 0; i < VP; ++i) {
+        int tok, x;
+        value_place(i, tok, x);
+        if (t0 + tok == pos) vr[i] = *reinterpret_cast<const uint4*>(vnew + x * 16);
+      }
     }
   };
 
@@ -139,9 +206,12 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const PagedAttnParam
   for (int d = 0; d < ND; ++d) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   int t0 = begin + wave * TOK;
-  int id = page_of(t0);
-  if (t0 < end) load_tile(t0, id);
-  id = page_of(t0 + 4 * TOK);
+  Ids ids;
+  if (t0 < end) {
+    ids = page_of(t0);
+    load_tile(t0, ids);
+    ids = page_of(t0 + 4 * TOK);
+  }
   for (; t0 < end; t0 += 4 * TOK) {
     const uint32_t ok = okmask;
     if (pos >= t0 && pos < t0 + TOK && sg == 0 && (ok >> (pos - t0) & 1u)) {  // the new token into its place
@@ -157,7 +227,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const PagedAttnParam
         }
 #pragma unroll
       for (int i = 0; i < VP; ++i) {
-        const int piece = i * 64 + lane, tok = piece / PIECES, x = piece - tok * PIECES;
+        int tok, x;
+        value_place(i, tok, x);
         if (t0 + tok == pos) *reinterpret_cast<uint4*>(vd + x * 16) = vr[i];
       }
     }
@@ -168,33 +239,50 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const PagedAttnParam
 #pragma unroll
       for (int i = 0; i < KP; ++i) s[u] = mma16<T>(kr[u][i], qf[i], s[u]);
     }
-    const bool whole = ok == (TOK == 32 ? 0xffffffffu : 0xffffu);
+    const bool whole = ok == ALL;
+    if (!whole) {                                      // what lies where no token is may be anything, NaN too
+#pragma unroll
+      for (int i = 0; i < VP; ++i) {
+        int tok, x;
+        value_place(i, tok, x);
+        if (!(ok >> tok & 1u)) vr[i] = make_uint4(0, 0, 0, 0);
+      }
+      asm volatile("");                                // (a branch, not a select in every tile)
+    }
 #pragma unroll
     for (int i = 0; i < VP; ++i) {
-      const int piece = i * 64 + lane, tok = piece / PIECES, x = piece - tok * PIECES;
-      if (!whole && !(ok >> tok & 1u)) vr[i] = make_uint4(0, 0, 0, 0);  // what lies where no token is may be anything, NaN too
+      int tok, x;
+      value_place(i, tok, x);
       *reinterpret_cast<uint4*>(vs + tok * VROW + x * (16 / (int)sizeof(T))) = vr[i];
     }
     if (t0 + 4 * TOK < end) {
-      load_tile(t0 + 4 * TOK, id);
-      id = page_of(t0 + 8 * TOK);
+      load_tile(t0 + 4 * TOK, ids);
+      ids = page_of(t0 + 8 * TOK);
     }
     // weights: this lane has head l15 and the tokens u * 16 + 4 quarter + i
     float top = m;
 #pragma unroll
+    for (int u = 0; u < NT; ++u) s[u] *= p.scale_log2e;
+    if (!whole) {
+#pragma unroll
+      for (int u = 0; u < NT; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!(ok >> (u * 16 + quarter * 4 + i) & 1u)) s[u][i] = -INFINITY;
+      asm volatile("");
+    }
+#pragma unroll
     for (int u = 0; u < NT; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[u][i] = (ok >> (u * 16 + quarter * 4 + i) & 1u) ? s[u][i] * p.scale_log2e : -INFINITY;
-        top = fmaxf(top, s[u][i]);
-      }
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    const float fac = __builtin_amdgcn_exp2f(m - top);
-    m = top;
-    l *= fac;
+      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[u][i]);
+    top = across_quarters_max(top);
+    if (__any(top > m)) {                              // (as a rule the maximum is found early)
+      const float fac = __builtin_amdgcn_exp2f(m - top);
+      m = top;
+      l *= fac;
 #pragma unroll
-    for (int d = 0; d < ND; ++d) o[d] *= fac;
+      for (int d = 0; d < ND; ++d) o[d] *= fac;
+    }
 #pragma unroll
     for (int u = 0; u < NT; ++u)
 #pragma unroll
@@ -331,8 +419,12 @@ static int launch_paged_attn(PagedAttnParams& p, hipStream_t st) {
   p.min_chunk = 128;
   const dim3 grid(p.splits, p.kv_heads * p.sub, p.rows);
   const int64_t pool = 2ll * p.pages * p.kv_heads * p.page.d * D * (int64_t)sizeof(T);
-  if (pool > kStreamBytes) paged_attn_kernel<T, D, true><<<grid, 256, 0, st>>>(p);
-  else paged_attn_kernel<T, D, false><<<grid, 256, 0, st>>>(p);
+  const bool groups = p.page.d % 16 == 0 && p.key_token * (int64_t)sizeof(T) < 1 << 26 && p.value_token * (int64_t)sizeof(T) < 1 << 26;  // (lane offsets of 32 bits)
+  const bool past = pool > kStreamBytes;
+  if (groups && past) paged_attn_kernel<T, D, true, true><<<grid, 256, 0, st>>>(p);
+  else if (groups) paged_attn_kernel<T, D, false, true><<<grid, 256, 0, st>>>(p);
+  else if (past) paged_attn_kernel<T, D, true, false><<<grid, 256, 0, st>>>(p);
+  else paged_attn_kernel<T, D, false, false><<<grid, 256, 0, st>>>(p);
   if (int rc = launch_status("paged_attention")) return rc;
   if (p.splits > 1) {
     paged_join_kernel<T, D><<<dim3(p.heads, p.rows), 256, 0, st>>>(p);
