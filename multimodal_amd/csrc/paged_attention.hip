@@ -395,18 +395,29 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
   }
 }
 
-// Splits of a row, from what the host knows: the rows, heads and the capacity of the page table (the lengths are on the device).
-static int paged_splits(int rows, int heads, int kv_heads, int64_t capacity) {
-  const int64_t wgs = (int64_t)rows * kv_heads;
-  int64_t s = (capacity + 1023) / 1024;
-  const int64_t fill = (2048 + wgs - 1) / wgs;
-  if (s < fill) s = fill;
-  const int64_t most = (capacity + 127) / 128;
+// Splits of a row, from what the host knows: the workgroups without splits (rows x key heads x 16s of a group) and the capacity of the page table (the lengths
+// are on the device; a kernel that finds a row shorter cuts it into fewer, of 128 tokens at least).  A split costs a second kernel, about 3 us.
+// Us a call, 12 heads of 64 in bf16, one split / more:
+//   one row        256 tokens 4.9 / 6.7, 512: 6.5 / 6.7, 1024: 9.6 / 7.0              -> one up to 64 KiB of keys a head
+//   32 rows        1024 tokens 18.4 / 21.5, 2048: 31.1 / 35.4, 4096: 73.7 / 74.8    -> one up to 256 KiB if there is a workgroup for every CU;
+//   61 rows, mixed up to 8192     stretches of 1024 tokens 66.9, of 2048: 69.9      -> beyond that, stretches of 1024: long rows must not end last
+//   5 rows         4096 tokens, 18 splits 16.9, 33: 16.6, 9: 18.7                     -> few rows: 1024 workgroups, stretches of 2048 at most
+static int paged_splits(int64_t wgs, int64_t capacity, int row_bytes) {
+  const int64_t whole = 65536 / row_bytes;
+  const bool full = wgs >= kChipCUs;
+  if (capacity <= (full ? 4 * whole : whole)) return 1;
+  int64_t s = full ? (capacity + 1023) / 1024 : (capacity + 2047) / 2048;
+  const int64_t fill = (1024 + wgs - 1) / wgs;
+  if (!full && s < fill) s = fill;
+  const int64_t most = (capacity + 127) / 128, grid = 16384 / wgs;
   if (s > most) s = most;
-  const int64_t grid = 16384 / wgs;
   if (s > grid) s = grid;
   if (s > kSplitsMost) s = kSplitsMost;
   return s < 1 ? 1 : (int)s;
+}
+static int paged_splits(const mmamd_paged_cache* c, int rows, int heads) {
+  const int64_t sub = (heads / c->kv_heads + 15) / 16;
+  return paged_splits((int64_t)rows * c->kv_heads * sub, (int64_t)c->slots * c->page_size, c->dim * (c->dtype == MMAMD_F32 ? 4 : 2));
 }
 
 // A pool of this size or less is read through the caches as usual, a larger one past them.  Us a call, as usual / past them: 1.07 GB 196.6 / 181.1; 322 MB
@@ -514,7 +525,7 @@ extern "C" int64_t mmamd_paged_attention_workspace(const mmamd_paged_cache* c, i
   if (int rc = check_pages("mmamd_paged_attention_workspace", c)) return rc;
   MMAMD_CHECK_ARG(rows >= 0 && heads >= 1 && heads % c->kv_heads == 0, MMAMD_E_BADARG, "mmamd_paged_attention_workspace: rows %d, heads %d, kv_heads %d", rows, heads, c->kv_heads);
   if (rows == 0) return 0;
-  const int s = paged_splits(rows, heads, c->kv_heads, (int64_t)c->slots * c->page_size);
+  const int s = paged_splits(c, rows, heads);
   return s == 1 ? 0 : (int64_t)rows * heads * s * (c->dim + 2) * 4;
 }
 
@@ -540,7 +551,7 @@ extern "C" int mmamd_paged_attention(const mmamd_paged_cache* c, const int32_t* 
   p.rows = rows; p.heads = heads; p.kv_heads = c->kv_heads; p.group = heads / c->kv_heads; p.pages = c->pages; p.slots = c->slots;
   p.page = fast_div((uint32_t)c->page_size);
   p.scale_log2e = scale * 1.4426950408889634f;
-  p.splits = paged_splits(rows, heads, c->kv_heads, (int64_t)c->slots * c->page_size);
+  p.splits = paged_splits(c, rows, heads);
   if (p.splits > 1) {
     const int64_t need = (int64_t)rows * heads * p.splits * (c->dim + 2) * 4;
     MMAMD_CHECK_ARG(workspace != nullptr && workspace_bytes >= need && aligned16(workspace), MMAMD_E_BADARG, "mmamd_paged_attention: workspace of %lld bytes, %lld needed",
