@@ -609,7 +609,7 @@ int mmamd_paged_attention(const mmamd_paged_cache* cache, const int32_t* lengths
                           int64_t k_row, int64_t k_head, const void* v, int64_t v_row, int64_t v_head, void* out, int rows, int heads, float scale,
                           void* workspace, int64_t workspace_bytes, mmamd_stream_t stream);
 /* Stores prompts: token j < counts[r] (counts NULL: all `tokens`) of row r, k / v [rows, tokens, kv_heads, dim] with any strides, goes to position
- * start[r] + j.  Tokens without a place are dropped; nothing else is written. */
+ * start[r] + j.  Tokens without a place are dropped; nothing else is written.  Two tokens must not go to one place. */
 int mmamd_paged_append(const mmamd_paged_cache* cache, const void* k, int64_t k_row, int64_t k_token, int64_t k_head, const void* v, int64_t v_row,
                        int64_t v_token, int64_t v_head, const int32_t* start, const int32_t* counts, int rows, int tokens, mmamd_stream_t stream);
 
@@ -634,7 +634,7 @@ int mmamd_paged_compact(void* pool, int pages, int64_t page_bytes, const int32_t
 
 /* One step of a beam search over groups x beams rows of logits [groups * beams, vocab] (fp32 or bf16, row stride ld).  A beam that goes on offers
  * scores[b] + log_softmax(logits[b])[v] for every v, a finished one its own score for v = eos; all others -inf.  The `beams` (<= 32) highest by
- * total / max(length, 1)^length_penalty (length: the continuation's) win, ties go to the lowest b * vocab + v.  A beam with score -inf or NaN, or whose
+ * total / max(length, 1)^length_penalty (finite; length: the continuation's) win, ties go to the lowest b * vocab + v.  A beam with score -inf or NaN, or whose
  * logits have no finite log-sum-exp (a NaN or +inf among them, or nothing but -inf), offers -inf throughout.
  * lengths int32, finished uint8, sequences int64 [groups, beams, tokens] (NULL: not kept) are reordered: outputs [groups, beams] each, out_parents the row
  * (group * beams + beam) that is continued -- paged_fork's `parents` --, out_sequences with the new token at the parent's length (dropped if there is no

@@ -60,7 +60,7 @@ __device__ __forceinline__ void beam_load4(const T* p, bool vec, int left, float
 // grid: ceil(units / 4) x rows, one unit a wave.  Of the lanes' maxima the `beams`-th highest is a bound that the unit's `beams` best do not fall below:
 // what lies above it (31 values for each of fewer than `beams` lanes, at most, a handful as a rule) and the first of its equals are gathered in LDS,
 // where each counts how many are better.  (Taking the best `beams` times over all 32 values of a lane was bound by its compares and shuffles: 39 us for
-// 512 rows of 49408, 12 us for 5.)
+// 512 rows of 49408, 12 us for 5; this way 18 and 6.)  Bound by HBM: 101 MB in 18 us, 5.6 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void beam_scan_kernel(const BeamParams p) {
   extern __shared__ uint2 lists[];
@@ -161,8 +161,8 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(const BeamParams p) {
 }
 
 // One workgroup per group.  A wave per beam joins the sums and merges the units' lists into the beam's `beams` best; the continuations of all beams then
-// count how many are better than they, which is their place.  Bound by its chain of dependent steps, so everything that can be loaded is loaded at once: a
-// row that was not scanned has whatever lay in the workspace, and does not use it.
+// count how many are better than they, which is their place.  Bound by its chain of dependent steps (6 to 7 us), so everything that can be loaded is loaded at
+// once: a row that was not scanned has whatever lay in the workspace, and does not use it.
 __global__ __launch_bounds__(512) void beam_join_kernel(const BeamParams p) {
   __shared__ double total[kBeamMost * kBeamMost];  // of the continuations of all beams: beam * beams + place
   __shared__ double rank[kBeamMost * kBeamMost];
@@ -260,9 +260,11 @@ __global__ __launch_bounds__(512) void beam_join_kernel(const BeamParams p) {
     }
     if (lane < K) {
       const double base = (double)(after > 1 ? after : 1);
-      rank[b * K + lane] = p.penalty == 0.0 ? total[b * K + lane] : total[b * K + lane] / (p.penalty == 1.0 ? base : pow(base, p.penalty));
+      const double r = p.penalty == 0.0 ? total[b * K + lane] : total[b * K + lane] / (p.penalty == 1.0 ? base : pow(base, p.penalty));
+      rank[b * K + lane] = r == r ? r : -INFINITY;       // (-inf over a power that overflows; every pair has to have an order)
     }
     if (lane < K) better[b * K + lane] = 0;
+    if (lane == 0) place[b] = 0;
     if (lane == 0) { fin[b] = done; len[b] = after; }
   }
   __syncthreads();
@@ -320,7 +322,7 @@ extern "C" int mmamd_beam_search_step(const void* logits, int dtype, int64_t ld,
   MMAMD_CHECK_ARG(dtype == MMAMD_F32 || dtype == MMAMD_BF16, MMAMD_E_UNSUPPORTED, "mmamd_beam_search_step: dtype code %d (fp32 / bf16 only)", dtype);
   MMAMD_CHECK_ARG(logits && scores && lengths && finished && out_scores && out_lengths && out_finished && out_tokens && out_parents && workspace && (sequences == nullptr) == (out_sequences == nullptr),
                   MMAMD_E_BADARG, "mmamd_beam_search_step: null argument");
-  MMAMD_CHECK_ARG(ld >= 0 && tokens >= 0 && eos >= 0 && eos < vocab && length_penalty == length_penalty, MMAMD_E_BADARG,
+  MMAMD_CHECK_ARG(ld >= 0 && tokens >= 0 && eos >= 0 && eos < vocab && length_penalty - length_penalty == 0.0, MMAMD_E_BADARG,
                   "mmamd_beam_search_step: ld %lld, tokens %d, eos %lld of a vocabulary of %d, length penalty %f", (long long)ld, tokens, (long long)eos, vocab, length_penalty);
   const int64_t need = mmamd_beam_search_workspace(groups, beams, vocab);
   MMAMD_CHECK_ARG(workspace_bytes >= need && aligned16(workspace), MMAMD_E_BADARG, "mmamd_beam_search_step: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);

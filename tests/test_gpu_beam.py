@@ -69,6 +69,9 @@ def test_first_step_and_dead_beams():
     finished[0] = True
     check(logits, torch.full_like(scores, float("-inf")), lengths, finished, seq, 7, 1.0)
     check(logits, torch.zeros_like(scores), lengths, torch.ones_like(finished), seq, 3, 1.0)
+    dead = torch.full_like(scores, float("-inf"))  # -inf over an infinite power has no order of its own: the lowest win
+    got = ops.beam_search_step(logits, dead, lengths + 1000, torch.zeros_like(finished), seq, 0, length_penalty=500.0)
+    assert host(got.tokens).tolist() == [[0, 1, 2, 3, 4]] * 2 and np.isneginf(host(got.scores)).all()
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])

@@ -84,7 +84,7 @@ def test_fork_compact_and_beam_arguments(L):
         return L.mmamd_beam_search_step(logits, dtype, ld, scores, 64, 64, seq, tokens, eos, penalty, groups, beams, vocab, out, 64, 64, 64, 64, out_seq, ws, size, None)
 
     for kw, code in [(dict(logits=None), -1), (dict(dtype=3), -2), (dict(beams=33), -2), (dict(beams=0), -1), (dict(groups=30000), -2), (dict(vocab=0), -1), (dict(eos=100), -1),
-                     (dict(eos=-1), -1), (dict(seq=64), -1), (dict(penalty=math.nan), -1), (dict(size=4), -1), (dict(ws=None), -1), (dict(out=None), -1), (dict(ld=-1), -1)]:
+                     (dict(eos=-1), -1), (dict(seq=64), -1), (dict(penalty=math.nan), -1), (dict(penalty=math.inf), -1), (dict(size=4), -1), (dict(ws=None), -1), (dict(out=None), -1), (dict(ld=-1), -1)]:
         assert beam(**kw) == code, kw
     assert beam(groups=0) == 0
 
@@ -117,6 +117,17 @@ def test_meta_kernels_infer_shapes():
     r = ns.beam_search_step(m(6, 50), m(2, 3), m(2, 3, dtype=i), m(2, 3, dtype=torch.bool), m(2, 3, 8, dtype=torch.int64), 1, 0.0)
     assert [t.dtype for t in r] == [torch.float32, i, torch.bool, torch.int64, i, torch.int64] and r[5].shape == (2, 3, 8)
     assert "Tensor(a!) key_pages" in str(ns.paged_attention.default._schema)
+
+
+def test_decoding_kernels_do_not_spill():
+    from concurrent.futures import ThreadPoolExecutor
+
+    from tools.check_spills import CSRC, check
+
+    with ThreadPoolExecutor(max_workers=3) as ex:
+        for name, rc, rows in ex.map(check, [CSRC / f for f in ("paged_attention.hip", "paged_pages.hip", "beam.hip")]):
+            assert rc == 0 and rows, name
+            assert not [r for r in rows if r[2] > 0 or r[1] > 256], name
 
 
 def test_page_division(tmp_path):
