@@ -45,6 +45,21 @@ __device__ __forceinline__ float dpp_max(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
+// a wave's sum, in every lane
+__device__ __forceinline__ double dpp_sum(double v) {
+#define MMAMD_DPP_ADD(ctrl, rows)                                                                                                                \
+  v += __hiloint2double(__builtin_amdgcn_update_dpp(0, __double2hiint(v), ctrl, rows, 0xf, false),                                              \
+                        __builtin_amdgcn_update_dpp(0, __double2loint(v), ctrl, rows, 0xf, false))
+  MMAMD_DPP_ADD(0x111, 0xf);
+  MMAMD_DPP_ADD(0x112, 0xf);
+  MMAMD_DPP_ADD(0x114, 0xf);
+  MMAMD_DPP_ADD(0x118, 0xf);
+  MMAMD_DPP_ADD(0x142, 0xa);
+  MMAMD_DPP_ADD(0x143, 0xc);
+#undef MMAMD_DPP_ADD
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), 63), __builtin_amdgcn_readlane(__double2loint(v), 63));
+}
+
 template <typename T>
 __device__ __forceinline__ void beam_load4(const T* p, bool vec, int left, float (&f)[4]) {
   if (vec && left >= 4) {
@@ -86,9 +101,7 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(const BeamParams p) {
   for (int i = 0; i < 8; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) part += __builtin_amdgcn_exp2f((f[i][j] - top) * 1.4426950408889634f);
-  double sum = top > -INFINITY ? (double)part : 0.0;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  double sum = dpp_sum(top > -INFINITY ? (double)part : 0.0);
   if (__any(!(part == part)) && top > -INFINITY) sum = NAN;
   const int64_t at = (int64_t)row * p.units + unit;
   if (top == -INFINITY) {  // nothing but -inf, or NaN and -inf: told apart here
@@ -199,9 +212,7 @@ __global__ __launch_bounds__(512) void beam_join_kernel(const BeamParams p) {
       top = dpp_max(top);
       double sum = m0 > -INFINITY ? s0 * exp((double)m0 - (double)top) : s0;
       for (int u = lane + 64; u < p.units; u += 64) sum += um[u] > -INFINITY ? us[u] * exp((double)um[u] - (double)top) : us[u];
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
-      lse = (double)top + log(sum);
+      lse = (double)top + log(dpp_sum(sum));
     }
     if (lse > -INFINITY && lse < INFINITY) {
       float v0 = INFINITY, mine = -INFINITY;  // the last one taken; lane k's: the k-th
