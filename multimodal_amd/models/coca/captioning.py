@@ -1,6 +1,7 @@
 """Captions from a CoCa model: the generative read-out of the decoder that the captioning loss trains (models/coca/coca_model.py:434-466 of the reference,
 which has none for it).  Beam search, one token of all beams per step, with the keys and values of both decoders in pages."""
-from typing import NamedTuple, Optional
+from threading import Lock
+from typing import Dict, NamedTuple, Optional
 
 import torch
 from torch import Tensor
@@ -27,6 +28,12 @@ def captioning_embeddings(model: CoCaModel, images: Tensor) -> Tensor:
     return pooled[0] if isinstance(pooled, list) else pooled[:, 1:]
 
 
+# A search with a graph has a stream of its own (the legacy default stream cannot be captured): one per device, since the allocator keeps what was freed per
+# stream, and new ones would each hold the caches of a search.  One search at a time is on it.
+_SEARCH_STREAMS: Dict[torch.device, torch.cuda.Stream] = {}
+_searching = Lock()
+
+
 class _Search:
     """The state of one search in tensors that stay where they are, so that a step can be captured in a HIP graph and replayed."""
 
@@ -46,7 +53,7 @@ class _Search:
         cross = self.fusion.transformer_decoder.cross_cache(states.contiguous(), page_size)
         self.caches[1].cross = cross.shared_rows(torch.arange(bsz, device=dev).repeat_interleave(beams))
         for cache in self.caches:
-            cache.fork(torch.full((rows,), -1, dtype=torch.int32, device=dev), reserve=1)
+            cache.fork(torch.full((rows,), -1, dtype=torch.int32, device=dev), reserve=1, cross=False)
         self.scores = torch.full((bsz, beams), float("-inf"), device=dev)
         self.scores[:, 0] = 0.0
         self.lengths = torch.zeros((bsz, beams), dtype=torch.int32, device=dev)
@@ -65,7 +72,7 @@ class _Search:
         for to, new in zip((self.scores, self.lengths, self.finished, self.tokens, self.sequences), (r.scores, r.lengths, r.finished, r.tokens, r.sequences)):
             to.copy_(new)
         for cache, held in zip(self.caches, self.held):
-            cache.fork(r.parents, reserve=1)
+            cache.fork(r.parents, reserve=1, cross=False)
             for to, new in zip(held, (cache.page_table, cache.lengths, cache.refcounts)):
                 to.copy_(new)
             cache.page_table, cache.lengths, cache.refcounts = held
@@ -99,7 +106,7 @@ def generate_captions(model: CoCaModel, images: Tensor, begin: int, end: int, nu
                       length_penalty: float = 1.0, page_size: int = 16, graph: bool = True) -> Captions:
     """Captions of images [bsz, ...] by beam search from token `begin` until every beam has taken `end` or has max_length tokens (default and at most: the
     text decoder's positions without its CLS).  Ranked by log-probability / length ** length_penalty.  graph: from the third token on a step is a replayed
-    HIP graph, in place of some three hundred launches from Python."""
+    HIP graph, in place of some three hundred launches from Python; such calls from several threads take turns."""
     if model.training:
         raise ops.MmamdError("generate_captions: call model.eval() first")
     text, fusion = model.text_decoder, model.multimodal_decoder
@@ -107,26 +114,41 @@ def generate_captions(model: CoCaModel, images: Tensor, begin: int, end: int, nu
     max_length = places if max_length is None else max_length
     if not 2 <= max_length <= places:
         raise ValueError(f"max_length must lie between 2 and the decoder's {places} positions, got {max_length}")
-    if num_beams < 1:
-        raise ValueError(f"num_beams must be at least 1, got {num_beams}")
+    if not 1 <= num_beams <= 32:
+        raise ValueError(f"num_beams must lie between 1 and 32 (ops.beam_search_step), got {num_beams}")
     if fusion.output_projection is None:
         raise ValueError("the multimodal decoder has no output projection to the vocabulary")
     vocab = text.embeddings.token_embeddings.num_embeddings
     if not (0 <= begin < vocab and 0 <= end < min(vocab, fusion.output_projection.out_features)) or fusion.output_projection.out_features > vocab:
         raise ValueError(f"begin {begin} and end {end} must be words of the vocabulary of {vocab}, which the output projection must not exceed")
+    if not images.is_cuda:
+        raise ops.MmamdError(f"generate_captions: the images are on {images.device}: the MI355X path needs HIP device tensors (no CPU fallback)")
     if images.shape[0] == 0:  # (the encoders take no empty batch)
         empty = torch.zeros((0, num_beams), device=images.device)
         return Captions(empty[:, :, None].expand(0, num_beams, max_length).long(), empty, empty.int())
-    states = captioning_embeddings(model, images)
-    main = torch.cuda.current_stream()
-    side = torch.cuda.Stream() if graph else main  # (the legacy default stream cannot be captured)
-    side.wait_stream(main)
-    with torch.cuda.stream(side):
-        search = _Search(model, states, begin, end, num_beams, max_length, length_penalty, page_size)
-        search.run(max_length - 1, graph)
+
+    def search() -> Captions:
+        s = _Search(model, states, begin, end, num_beams, max_length, length_penalty, page_size)
+        s.run(max_length - 1, graph)
         first = torch.full((states.shape[0], num_beams, 1), begin, dtype=torch.int64, device=states.device)
-        result = Captions(torch.cat([first, search.sequences], dim=2), search.scores, search.lengths)
-    main.wait_stream(side)
-    for t in (*result, states):
-        t.record_stream(main)
-    return result
+        return Captions(torch.cat([first, s.sequences], dim=2), s.scores, s.lengths)
+
+    with torch.cuda.device(images.device):
+        if not graph:
+            states = captioning_embeddings(model, images)
+            return search()
+        with _searching:
+            states = captioning_embeddings(model, images)
+            main = torch.cuda.current_stream()
+            side = _SEARCH_STREAMS.get(states.device)
+            if side is None:
+                side = _SEARCH_STREAMS[states.device] = torch.cuda.Stream(states.device)
+            side.wait_stream(main)
+            try:
+                with torch.cuda.stream(side):
+                    result = search()
+            finally:
+                main.wait_stream(side)
+        for t in result:
+            t.record_stream(main)
+        return result

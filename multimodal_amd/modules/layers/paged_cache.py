@@ -33,11 +33,13 @@ class PagedKVCache:
             raise ValueError("n_layer, num_heads, num_pages, max_tokens and page_size must be at least 1")
         self.page_size, self.max_tokens = page_size, max_tokens
         self.pages = torch.empty((num_pages, n_layer, 2, num_heads, page_size, head_dim), dtype=dtype, device=device)
-        self.cross: Optional["PagedKVCache"] = None  # keys and values of encoder states, for decoders with cross-attention
+        self.cross: Optional["PagedKVCache"] = None  # keys and values of encoder states, for decoders with cross-attention, row for row
+        self._view = False
         self.reset()
 
     def reset(self) -> None:
         """No rows, every page free."""
+        self._owned("reset")
         dev = self.pages.device
         slots = -(-self.max_tokens // self.page_size)
         self.page_table = torch.empty((0, slots), dtype=torch.int32, device=dev)
@@ -54,51 +56,82 @@ class PagedKVCache:
     def n_layer(self) -> int:
         return self.pages.shape[1]
 
+    def _owned(self, what: str) -> None:
+        if self._view:
+            raise ops.MmamdError(f"{what}: shared_rows() reads the pages of another cache and holds no references to them")
+
     def layer(self, i: int) -> Tuple[Tensor, Tensor]:
         """(key_pages, value_pages) of layer i, views [num_pages, num_heads, page_size, head_dim]."""
         return self.pages[:, i, 0], self.pages[:, i, 1]
 
     def add_rows(self, rows: int, tokens: Union[int, Tensor]) -> None:
         """`rows` new rows in the place of the present ones (which must be none, or are dropped), with pages for prompts of `tokens` tokens (an int, or
-        int32 [rows]); the next decoder call stores them."""
-        self.fork(torch.full((rows,), -1, dtype=torch.int32, device=self.pages.device), reserve=tokens)
+        int32 [rows]); the next decoder call stores them.  `cross` stays as it is: assign the new rows' before or after."""
+        room = self.page_table.shape[1] * self.page_size
+        if isinstance(tokens, int) and tokens > room:
+            raise ValueError(f"prompts of {tokens} tokens for rows of {room}")
+        self.fork(torch.full((rows,), -1, dtype=torch.int32, device=self.pages.device), reserve=tokens, cross=False)
         self._prompt = tokens
 
-    def fork(self, parents: Tensor, reserve: Union[int, Tensor] = 1) -> None:
-        """Row r becomes a continuation of the present row parents[r] (int32, any shape, -1: an empty row) with room for `reserve` more tokens."""
+    def fork(self, parents: Tensor, reserve: Union[int, Tensor] = 1, cross: bool = True) -> None:
+        """Row r becomes a continuation of the present row parents[r] (int32, any shape, -1: an empty row) with room for `reserve` more tokens.  The rows of
+        `cross` follow (the row of an empty one has no states); cross=False leaves them, where a row and its parent have the same states in any case."""
+        self._owned("fork")
+        if cross and self.cross is not None:
+            if self.cross.rows != self.rows:
+                raise ValueError(f"the encoder states' cache has {self.cross.rows} rows, this one {self.rows}")
+            follow = self.cross._continued(parents.reshape(-1))
+        else:
+            follow = self.cross
         s = ops.paged_fork(self.pages, self.page_table, self.lengths, self.refcounts, parents.reshape(-1), reserve=reserve)
         self.page_table, self.lengths, self.refcounts, self.shortage = s
+        self.cross = follow
         self._prompt = None
 
     def reserve(self, tokens: Union[int, Tensor] = 1) -> None:
         """Room for `tokens` more tokens in every row."""
-        self.fork(torch.arange(self.rows, dtype=torch.int32, device=self.pages.device), reserve=tokens)
+        self.fork(torch.arange(self.rows, dtype=torch.int32, device=self.pages.device), reserve=tokens, cross=False)
 
     def shared_rows(self, parents: Tensor) -> "PagedKVCache":
-        """Another view of the same pages: its row r reads what row parents[r] (int64) holds now.  For reading only -- it takes no references, so nothing may be
-        stored, forked or compacted through it, and this cache has to keep the rows."""
+        """Another view of the same pages: its row r reads what row parents[r] (int64) holds now.  For reading only -- it takes no references, so storing, forking
+        and compacting through it are refused, and this cache has to keep the rows where they are (no fork that drops them, no compact or resize)."""
         view = object.__new__(PagedKVCache)
         view.__dict__.update(self.__dict__)
-        view.page_table, view.lengths = self.page_table[parents], self.lengths[parents]
+        view.page_table, view.lengths, view._view = self.page_table[parents], self.lengths[parents], True
+        return view
+
+    def _continued(self, parents: Tensor) -> "PagedKVCache":
+        """shared_rows() for fork's parents: a number outside the rows gives a row without tokens."""
+        if self.rows == 0:
+            view = self.shared_rows(torch.zeros((0,), dtype=torch.int64, device=parents.device))
+            view.page_table, view.lengths = view.page_table.new_full((len(parents), view.page_table.shape[1]), -1), view.lengths.new_zeros((len(parents),))
+            return view
+        view = self.shared_rows(parents.clamp(0, self.rows - 1).long())
+        view.lengths = torch.where((parents >= 0) & (parents < self.rows), view.lengths, 0)
         return view
 
     def append(self, layer: int, k: Tensor, v: Tensor, counts: Optional[Tensor] = None) -> None:
         """Stores k, v [rows, tokens, num_heads, head_dim] (counts int32 [rows]: the first ones of each row) behind the rows' tokens; advance() is the caller's."""
+        self._owned("append")
         kp, vp = self.layer(layer)
         ops.paged_append(k, v, kp, vp, self.page_table, self.lengths, counts)
 
     def attend(self, layer: int, q: Tensor, k: Optional[Tensor] = None, v: Optional[Tensor] = None, scale: Optional[float] = None) -> Tensor:
         """One token a row: q [rows, heads, head_dim] over the row's tokens in `layer`, and over its new one, which is stored, if k and v are given."""
+        if k is not None:
+            self._owned("attend with new tokens")
         kp, vp = self.layer(layer)
         return ops.paged_attention(q, kp, vp, self.page_table, self.lengths, k, v, scale)
 
     def advance(self, tokens: Union[int, Tensor] = 1) -> None:
         """Counts tokens that every layer has stored."""
+        self._owned("advance")
         self.lengths = self.lengths + tokens
         self._prompt = None
 
     def compact(self) -> int:
         """Moves the live pages to the front and says how many they are (this waits for the device)."""
+        self._owned("compact")
         self.page_table, self.refcounts, live = ops.paged_compact(self.pages, self.page_table, self.refcounts)
         return int(live)
 

@@ -557,7 +557,7 @@ def _decoder_forward_paged(self, hidden_states: Tensor, encoder_hidden_states, c
         if return_hidden_states:
             hidden.append(x.view(B, S, d))
         x = layer_module.run_paged(x, B, S, cache, i, enc, Sk)
-    cache.advance(1 if prompt is None else prompt)
+    cache.advance(1 if prompt is None else prompt if isinstance(prompt, int) else prompt.clamp(0, S))  # (a count beyond the prompt has stored nothing there)
     x = x.view(B, S, d)
     if return_hidden_states:
         hidden.append(x)

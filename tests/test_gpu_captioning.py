@@ -174,3 +174,84 @@ def test_captions_vs_full_forward(cfg, cascaded):
     model.train()
     with pytest.raises(RuntimeError):
         generate_captions(model, images, 1, end)
+
+
+@torch.no_grad()
+def test_rows_with_their_own_encoder_states_reordered():
+    """Forked rows keep attending to their parents' encoder states: each equals the causal pass of its tokens beside the states it began with."""
+    from multimodal_amd.modules.layers.transformer import TransformerDecoder
+
+    torch.manual_seed(2)
+    dec = TransformerDecoder(n_layer=2, d_model=128, n_head=2, dim_feedforward=256, activation=torch.nn.GELU, layer_norm_eps=1e-5, norm_first=True,
+                             use_cross_attention=True, dim_kv=128).cuda().eval()
+    g = torch.Generator().manual_seed(3)
+    enc, rows = 3.0 * torch.randn(3, 9, 128, generator=g).cuda(), [torch.randn(4, 128, generator=g) for _ in range(3)]
+    cache = cache_for(dec, 6, 16, 4)
+    cache.add_rows(3, 4)
+    dec(torch.stack(rows).cuda(), enc, past_key_values=cache)
+    cache.cross, of = dec.cross_cache(enc, 4), [0, 1, 2]
+    for parents in ([2, 0, 0, 1], [3, 1, 0]):
+        cache.fork(torch.tensor(parents, dtype=torch.int32, device="cuda"))
+        new = torch.randn(len(parents), 1, 128, generator=g)
+        rows, of = [torch.cat([rows[p], x]) for p, x in zip(parents, new)], [of[p] for p in parents]
+        got = dec(new.cuda(), past_key_values=cache).last_hidden_state[:, 0]
+        want = dec(torch.stack(rows).cuda(), enc[of], attention_mask=causal(len(rows[0]))).last_hidden_state[:, -1]
+        other = dec(torch.stack(rows).cuda(), enc[[(o + 1) % 3 for o in of]], attention_mask=causal(len(rows[0]))).last_hidden_state[:, -1]
+        assert np.abs(host(got) - host(want)).max() <= 2e-2
+        assert np.abs(host(other) - host(want)).max() > 0.2  # (the states matter)
+
+
+@torch.no_grad()
+def test_prompt_counts_beyond_the_prompt():
+    """A count above the prompt's padded length counts what was stored, no places that were never written."""
+    from multimodal_amd.modules.layers.transformer import TransformerDecoder
+
+    torch.manual_seed(4)
+    dec = TransformerDecoder(n_layer=1, d_model=128, n_head=2, dim_feedforward=256, activation=torch.nn.GELU, layer_norm_eps=1e-5, norm_first=True,
+                             use_cross_attention=False).cuda().eval()
+    x = torch.randn(3, 6, 128, generator=torch.Generator().manual_seed(5)).cuda()
+    last = []
+    for counts in ([9, 3, -2], [5, 3, 0]):
+        cache = cache_for(dec, 3, 16, 4)
+        cache.pages.fill_(float("nan"))
+        cache.add_rows(3, torch.tensor(counts, dtype=torch.int32, device="cuda"))
+        dec(x[:, :5], past_key_values=cache)
+        assert host(cache.lengths).tolist() == [5, 3, 0]
+        cache.reserve(1)
+        last.append(dec(x[:, 5:], past_key_values=cache).last_hidden_state)
+    assert torch.equal(last[0], last[1]) and bool(torch.isfinite(last[0]).all())
+
+
+@torch.no_grad()
+def test_captions_of_two_streams_and_two_threads():
+    """Calls that follow each other on different streams without a wait, and calls from two threads, give what single calls give."""
+    from threading import Thread
+
+    from multimodal_amd.models.coca.captioning import generate_captions
+
+    model = coca(SMALL, False, 62)
+    g = torch.Generator().manual_seed(6)
+    images = [torch.randn(2, 3, 64, 64, generator=g).cuda() for _ in range(2)]
+    want = [generate_captions(model, x, 1, 2, num_beams=3) for x in images]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [None, None]
+
+    def call(i):
+        with torch.no_grad(), torch.cuda.stream(streams[i]):
+            got[i] = generate_captions(model, images[i], 1, 2, num_beams=3)
+
+    def check():
+        torch.cuda.synchronize()
+        for w, r in zip(want, got):
+            assert torch.equal(w.sequences, r.sequences) and torch.equal(w.scores, r.scores) and torch.equal(w.lengths, r.lengths)
+        got[:] = [None, None]
+
+    for i in range(2):
+        call(i)
+    check()
+    threads = [Thread(target=call, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    check()

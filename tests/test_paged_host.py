@@ -234,3 +234,63 @@ def test_cache_and_captioning_arguments():
     for kw in (dict(max_length=1), dict(max_length=13), dict(num_beams=0), dict(begin=96), dict(end=-1)):
         with pytest.raises(ValueError):
             generate_captions(model, images, **{"begin": 1, "end": 2, **kw})
+
+
+def test_a_view_of_shared_rows_stores_and_moves_nothing():
+    """shared_rows() holds no references: what would write or reassign pages through it is refused."""
+    from multimodal_amd import ops
+    from multimodal_amd.modules.layers.paged_cache import PagedKVCache
+
+    cache = PagedKVCache(1, 2, 64, 5, 33, 16, device="cpu")
+    cache.page_table, cache.lengths = torch.tensor([[0, 1, -1], [2, -1, -1]], dtype=torch.int32), torch.tensor([20, 3], dtype=torch.int32)
+    view = cache.shared_rows(torch.tensor([1, 1, 0]))
+    assert view.page_table.tolist() == [[2, -1, -1], [2, -1, -1], [0, 1, -1]] and view.lengths.tolist() == [3, 3, 20] and view.pages is cache.pages
+    kv, rows = torch.zeros(3, 2, 64, dtype=torch.bfloat16), torch.zeros(3, dtype=torch.int32)
+    for call in (lambda: view.fork(rows), lambda: view.reserve(1), lambda: view.add_rows(1, 1), lambda: view.append(0, kv[:, None], kv[:, None]),
+                 lambda: view.attend(0, kv, kv, kv), view.advance, view.compact, lambda: view.resize(5), view.reset):
+        with pytest.raises(ops.MmamdError, match="another cache"):
+            call()
+    assert view.lengths.tolist() == [3, 3, 20] and cache.lengths.tolist() == [20, 3]
+
+
+def test_rows_of_encoder_states_follow_a_fork(monkeypatch):
+    """fork() takes the rows of `cross` along (on the CPU: the operator is replaced by its oracle's table)."""
+    from multimodal_amd import ops
+    from multimodal_amd.modules.layers.paged_cache import PagedKVCache
+
+    cache, cross = (PagedKVCache(1, 2, 64, 8, 33, 16, device="cpu") for _ in range(2))
+
+    def fork(pages, table, lengths, refcounts, parents, reserve):
+        n = len(parents)
+        return ops.PagedState(torch.full((n, 3), -1, dtype=torch.int32), torch.zeros(n, dtype=torch.int32), refcounts, torch.zeros(1, dtype=torch.int32))
+
+    monkeypatch.setattr(ops, "paged_fork", fork)
+    cross.page_table, cross.lengths = torch.tensor([[0, 1, -1], [2, -1, -1]], dtype=torch.int32), torch.tensor([20, 3], dtype=torch.int32)
+    cache.cross = cross
+    with pytest.raises(ValueError, match="2 rows, this one 0"):
+        cache.fork(torch.tensor([-1, -1], dtype=torch.int32))
+    cache.add_rows(2, 4)
+    assert cache.cross is cross and cache.rows == 2
+    cache.fork(torch.tensor([1, -1, 0, 7], dtype=torch.int32))
+    assert cache.cross.lengths.tolist() == [3, 0, 20, 0] and cache.cross.page_table[[0, 2]].tolist() == [[2, -1, -1], [0, 1, -1]]
+    cache.reserve(2)
+    assert cache.cross.lengths.tolist() == [3, 0, 20, 0]
+    cache.fork(torch.tensor([[2], [0]], dtype=torch.int32))
+    assert cache.cross.lengths.tolist() == [20, 3] and cross.lengths.tolist() == [20, 3] and cross.rows == 2
+    held = cache.cross
+    cache.fork(torch.tensor([0, 0, 0], dtype=torch.int32), cross=False)
+    assert cache.cross is held
+
+
+def test_prompts_beyond_the_table_and_beams_beyond_the_kernel_are_refused():
+    from multimodal_amd.models.coca.captioning import generate_captions
+    from multimodal_amd.models.coca.coca_model import coca_vit
+    from multimodal_amd.modules.layers.paged_cache import PagedKVCache
+    from tests.golden.make_golden_coca import SMALL
+
+    cache = PagedKVCache(1, 2, 64, 5, 33, 16, device="cpu")
+    with pytest.raises(ValueError, match="49 tokens for rows of 48"):
+        cache.add_rows(2, 49)
+    model = coca_vit(**SMALL, cascaded_pooler=False).eval()
+    with pytest.raises(ValueError, match="between 1 and 32"):
+        generate_captions(model, torch.zeros(1, 3, 64, 64), 1, 2, num_beams=33)
