@@ -1451,7 +1451,9 @@ def _decoding():
 
 
 def _refused(name: str, e: Exception, tensors) -> MmamdError:
-    """The error of a dispatcher op in the form the other wrappers raise."""
+    """The error of a dispatcher op in the form the other wrappers raise (out of memory stays what it is)."""
+    if isinstance(e, torch.OutOfMemoryError):
+        raise e
     for t in tensors:
         if isinstance(t, torch.Tensor) and not t.is_cuda and t.device.type != "meta":
             return MmamdError(f"{name}: a tensor is on {t.device}: the MI355X path needs HIP device tensors (no CPU fallback)")
@@ -1466,7 +1468,7 @@ def paged_attention(q: torch.Tensor, key_pages: torch.Tensor, value_pages: torch
     q [rows, heads, dim]; key_pages / value_pages [pages, kv_heads, page_size, dim] (any strides, dim contiguous; dim 64, 96 or 128; bf16 or fp32, the same
     for all), heads a multiple of kv_heads; page_table int32 [rows, slots]; lengths int32 [rows] = tokens a row has in the cache.  With k, v [rows, kv_heads,
     dim] the new token is stored at position lengths[row] and seen; lengths are the caller's to advance.  Page numbers outside the pool hold no
-    tokens; a row that sees nothing gives zeros.  scale: 1 / sqrt(dim) unless given.  Two rows' new tokens must not share a place.  out: a contiguous
+    tokens; a row that sees nothing gives zeros.  Places that hold no token may hold anything; an infinite or NaN value of a token makes the outputs it reaches NaN.  scale: 1 / sqrt(dim) unless given.  Two rows' new tokens must not share a place.  out: a contiguous
     tensor for the result.  All tensors on one device, on whose current stream the work is put."""
     try:
         if out is None:

@@ -294,3 +294,28 @@ def test_prompts_beyond_the_table_and_beams_beyond_the_kernel_are_refused():
     model = coca_vit(**SMALL, cascaded_pooler=False).eval()
     with pytest.raises(ValueError, match="between 1 and 32"):
         generate_captions(model, torch.zeros(1, 3, 64, 64), 1, 2, num_beams=33)
+
+
+def test_out_of_memory_keeps_its_type(monkeypatch):
+    """Callers free memory and go on where they catch torch.OutOfMemoryError."""
+    from multimodal_amd import ops
+
+    def full(*args):
+        raise torch.OutOfMemoryError("out of memory")
+
+    def wrong(*args):
+        raise RuntimeError("a reason\nand a trace")
+
+    pages, table, ints = torch.zeros(2, 1, 4, 64, device="meta"), torch.zeros(1, 1, dtype=torch.int32, device="meta"), torch.zeros(1, dtype=torch.int32, device="meta")
+    q, logits, scores = torch.zeros(1, 1, 64, device="meta"), torch.zeros(1, 4, device="meta"), torch.zeros(1, 1, device="meta")
+    calls = {"paged_attention": lambda: ops.paged_attention(q, pages, pages, table, ints), "paged_attention_into": lambda: ops.paged_attention(q, pages, pages, table, ints, out=q),
+             "paged_append": lambda: ops.paged_append(q[None], q[None], pages, pages, table, ints), "paged_fork": lambda: ops.paged_fork(pages, table, ints, ints, ints),
+             "paged_compact": lambda: ops.paged_compact(pages, table, ints),
+             "beam_search_step": lambda: ops.beam_search_step(logits, scores, ints[None], ints[None].bool(), None, 0)}
+    for name, call in calls.items():
+        monkeypatch.setattr(ops, "_DECODING", {name: full})
+        with pytest.raises(torch.OutOfMemoryError):
+            call()
+        monkeypatch.setattr(ops, "_DECODING", {name: wrong})
+        with pytest.raises(ops.MmamdError, match="^a reason$"):
+            call()
