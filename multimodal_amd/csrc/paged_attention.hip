@@ -356,7 +356,8 @@ __global__ __launch_bounds__(256, 2) void paged_attn_kernel(const PagedAttnParam
 }
 
 // Joins the splits of a (row, head): o = sum_s 2^(m_s - m) o_s / sum_s 2^(m_s - m) l_s.  The statistics of all splits first, one a thread; then the
-// outputs, each group of D threads every NG-th split, whose loads do not wait for one another.
+// outputs, each group of D threads every NG-th split, whose loads do not wait for one another.  The first of them are requested before the statistics are joined: 61
+// rows of up to 8192 tokens 67.15 -> 66.65 us a call; the kernel takes 4 to 5, a chain of loads.
 constexpr int kSplitsMost = 256;
 template <typename T, int D>
 __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p) {
@@ -371,6 +372,15 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
   if (n <= chunk) return;                               // a single split has written its output
   const int used = (n + chunk - 1) / chunk;
   if (tid >= used) ml = make_float2(-3.402823466e38f, 0.f);  // (what nobody wrote)
+  const int g = tid / D, d = tid - g * D;
+  const float* const o = p.ws + rh * p.splits * D + d;
+  constexpr int AHEAD = 8;                              // outputs that are requested before the statistics are there
+  float ahead[AHEAD];
+#pragma unroll
+  for (int k = 0; k < AHEAD; ++k) {
+    const int s = g + k * NG;
+    ahead[k] = o[(int64_t)(g < NG && s < used ? s : 0) * D];
+  }
   float top = wave_max(ml.x);
   if (lane == 0) red[wave] = top;
   __syncthreads();
@@ -380,12 +390,13 @@ __global__ __launch_bounds__(256) void paged_join_kernel(const PagedAttnParams p
   const float ls = wave_sum(ml.y * f);
   if (lane == 0) sums[wave] = ls;
   __syncthreads();
-  const int g = tid / D, d = tid - g * D;
   if (g < NG) {
-    const float* o = p.ws + rh * p.splits * D + d;
     float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (g + k * NG < used) v = fmaf(w[g + k * NG], ahead[k], v);
 #pragma unroll 8
-    for (int s = g; s < used; s += NG) v = fmaf(w[s], o[(int64_t)s * D], v);
+    for (int s = g + AHEAD * NG; s < used; s += NG) v = fmaf(w[s], o[(int64_t)s * D], v);
     part[g][d] = v;
   }
   __syncthreads();

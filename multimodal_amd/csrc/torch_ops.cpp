@@ -478,11 +478,11 @@ namespace {
 using OptTensor = c10::optional<Tensor>;
 
 // one call's view of its tensors: all on the device of the first, which becomes the current one
-struct Checker {
+struct ArgCheck {
   const char* who;
   at::Device device;
   c10::hip::HIPGuardMasqueradingAsCUDA guard;
-  Checker(const char* w, const Tensor& t) : who(w), device(t.device()), guard(t.device()) {}
+  ArgCheck(const char* w, const Tensor& t) : who(w), device(t.device()), guard(t.device()) {}
   // -1 in `shape`: any size; contiguous in the last axis, or altogether where `whole`
   void operator()(const Tensor& t, const char* name, at::ScalarType dt, at::IntArrayRef shape, bool whole = false) const {
     TORCH_CHECK(t.is_cuda(), who, ": ", name, " is on ", t.device(), ": the MI355X path needs HIP device tensors (no CPU fallback)");
@@ -498,7 +498,7 @@ struct Checker {
 // an axis of one entry is never stepped along, whatever its stride says
 int64_t step(const Tensor& t, int64_t axis) { return t.size(axis) > 1 ? t.stride(axis) : 0; }
 
-mmamd_paged_cache paged_cache(const Checker& ck, const Tensor& keys, const Tensor& values, const Tensor& table, int64_t rows) {
+mmamd_paged_cache paged_cache(const ArgCheck& ck, const Tensor& keys, const Tensor& values, const Tensor& table, int64_t rows) {
   const at::ScalarType dt = keys.scalar_type();
   TORCH_CHECK(dt == at::kFloat || dt == at::kBFloat16, ck.who, ": key_pages must be float32 or bfloat16, got ", dt);
   ck(keys, "key_pages", dt, {-1, -1, -1, -1});
@@ -525,7 +525,7 @@ int32_t* iptr(const Tensor& t) { return (int32_t*)ptr(t); }
 
 void paged_attention_into(const Tensor& q, const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& lengths, const OptTensor& k, const OptTensor& v,
                           c10::optional<double> scale, const Tensor& out) {
-  const Checker ck("paged_attention", keys);
+  const ArgCheck ck("paged_attention", keys);
   TORCH_CHECK(q.dim() == 3, "paged_attention: q must be a [rows, heads, dim] tensor");
   const int64_t rows = q.size(0), heads = q.size(1);
   const mmamd_paged_cache c = paged_cache(ck, keys, values, table, rows);
@@ -559,7 +559,7 @@ Tensor paged_attention_meta(const Tensor& q, const Tensor&, const Tensor&, const
 void paged_attention_into_meta(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptTensor&, const OptTensor&, c10::optional<double>, const Tensor&) {}
 
 void paged_append_impl(const Tensor& k, const Tensor& v, const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& start, const OptTensor& counts) {
-  const Checker ck("paged_append", keys);
+  const ArgCheck ck("paged_append", keys);
   TORCH_CHECK(k.dim() == 4, "paged_append: k must be a [rows, tokens, kv_heads, dim] tensor");
   const int64_t rows = k.size(0), tokens = k.size(1);
   const mmamd_paged_cache c = paged_cache(ck, keys, values, table, rows);
@@ -575,7 +575,7 @@ void paged_append_impl(const Tensor& k, const Tensor& v, const Tensor& keys, con
 }
 void paged_append_meta(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptTensor&) {}
 
-void check_pool(const Checker& ck, const Tensor& pages, const Tensor& refcounts, const Tensor& table) {
+void check_pool(const ArgCheck& ck, const Tensor& pages, const Tensor& refcounts, const Tensor& table) {
   TORCH_CHECK(pages.scalar_type() == at::kFloat || pages.scalar_type() == at::kBFloat16, ck.who, ": pages must be float32 or bfloat16, got ", pages.scalar_type());
   TORCH_CHECK(pages.dim() >= 3, ck.who, ": pages must be a [pages, ..., page_size, dim] tensor, got ", pages.sizes());
   ck(pages, "pages", pages.scalar_type(), pages.sizes(), true);
@@ -588,7 +588,7 @@ at::TensorOptions ints(const Tensor& t) { return t.options().dtype(at::kInt); }
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> paged_fork_impl(const Tensor& pages, const Tensor& table, const Tensor& lengths, const Tensor& refcounts, const Tensor& parents,
                                                            const OptTensor& reserve_rows, int64_t reserve) {
-  const Checker ck("paged_fork", pages);
+  const ArgCheck ck("paged_fork", pages);
   check_pool(ck, pages, refcounts, table);
   ck(lengths, "lengths", at::kInt, {table.size(0)});
   ck(parents, "parents", at::kInt, {-1});
@@ -611,7 +611,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> paged_fork_meta(const Tensor& pages, 
 }
 
 std::tuple<Tensor, Tensor, Tensor> paged_compact_impl(const Tensor& pages, const Tensor& table, const Tensor& refcounts) {
-  const Checker ck("paged_compact", pages);
+  const ArgCheck ck("paged_compact", pages);
   check_pool(ck, pages, refcounts, table);
   const int64_t n = pages.size(0);
   Tensor new_table = at::empty(table.sizes(), ints(pages)), counts = at::empty({n}, ints(pages)), live = at::empty({1}, ints(pages));
@@ -635,7 +635,7 @@ BeamOut beam_outputs(const Tensor& scores, const OptTensor& sequences) {
 // (without sequences the last output is empty: the schema has no optional returns that every caller could unpack)
 BeamOut beam_search_step_impl(const Tensor& logits, const Tensor& scores, const Tensor& lengths, const Tensor& finished, const OptTensor& sequences, int64_t eos,
                               double length_penalty) {
-  const Checker ck("beam_search_step", logits);
+  const ArgCheck ck("beam_search_step", logits);
   const at::ScalarType dt = logits.scalar_type();
   TORCH_CHECK(dt == at::kFloat || dt == at::kBFloat16, "beam_search_step: logits must be float32 or bfloat16, got ", dt);
   ck(scores, "scores", at::kFloat, {-1, -1}, true);
