@@ -45,6 +45,20 @@ __device__ __forceinline__ float dpp_max(float v) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63));
 }
 
+__device__ __forceinline__ double dpp_max(double v) {
+#define MMAMD_DPP_MAX(ctrl, rows)                                                                                                                     \
+  v = fmax(v, __hiloint2double(__builtin_amdgcn_update_dpp(__double2hiint(v), __double2hiint(v), ctrl, rows, 0xf, false),                             \
+                               __builtin_amdgcn_update_dpp(__double2loint(v), __double2loint(v), ctrl, rows, 0xf, false)))
+  MMAMD_DPP_MAX(0x111, 0xf);
+  MMAMD_DPP_MAX(0x112, 0xf);
+  MMAMD_DPP_MAX(0x114, 0xf);
+  MMAMD_DPP_MAX(0x118, 0xf);
+  MMAMD_DPP_MAX(0x142, 0xa);
+  MMAMD_DPP_MAX(0x143, 0xc);
+#undef MMAMD_DPP_MAX
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), 63), __builtin_amdgcn_readlane(__double2loint(v), 63));
+}
+
 // a wave's sum, in every lane
 __device__ __forceinline__ double dpp_sum(double v) {
 #define MMAMD_DPP_ADD(ctrl, rows)                                                                                                                \
@@ -173,38 +187,86 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(const BeamParams p) {
   if (lane >= n && lane < K) out[lane] = make_uint2(0xff800000u, 0xffffffffu);  // none
 }
 
-// One workgroup per group.  A wave per beam joins the sums and merges the units' lists into the beam's `beams` best; the continuations of all beams then
-// count how many are better than they, which is their place.  Bound by its chain of dependent steps (6 to 7 us), so everything that can be loaded is loaded at
-// once: a row that was not scanned has whatever lay in the workspace, and does not use it.
-__global__ __launch_bounds__(512) void beam_join_kernel(const BeamParams p) {
+// The `beams` best of a row, from the units' lists: each is in order, so the best that is left is at one of their heads.  A lane watches M neighbouring units,
+// so that of equal logits the lowest lane's is the lowest word.  stage: the first S of every list, in LDS; the rest is read where it lies.  Lane k gets the k-th.
+constexpr int kBeamStage = 256;
+// Up to this many beams every pair of a group's continuations is compared at once (beams^4 pairs), beyond it the beams' lists are put in order and merged.  Us a
+// call, 25 groups of 49408 words, pairs / merged: 4 beams 16.1 / 17.0, 5: 18.3 / 19.3, 8: 27.1 / 23.8, 9: 33.7 / 25.7.
+constexpr int kBeamPairs = 6;
+template <int M>
+__device__ __forceinline__ int merge_units(const uint2* list, const uint2* stage, int units, int S, int K, int lane, float& mine, uint32_t& word) {
+  float hv[M];
+  uint32_t hi[M];
+  int pos[M];
+#pragma unroll
+  for (int j = 0; j < M; ++j) {
+    const int u = lane * M + j;
+    const uint2 e = u < units ? stage[u * S] : make_uint2(0xff800000u, 0xffffffffu);
+    hv[j] = __uint_as_float(e.x);
+    hi[j] = e.y;
+    pos[j] = 0;
+  }
+  int found = 0;
+  for (; found < K; ++found) {
+    float bv = hv[0];
+    uint32_t bi = hi[0];
+    int bj = 0;
+#pragma unroll
+    for (int j = 1; j < M; ++j)
+      if (hv[j] > bv) { bv = hv[j]; bi = hi[j]; bj = j; }
+    const float best = dpp_max(bv);
+    if (!(best > -INFINITY)) break;
+    const int win = __ffsll((unsigned long long)__ballot(bv == best)) - 1;
+    const uint32_t low = (uint32_t)__builtin_amdgcn_readlane((int)bi, win);
+    if (lane == found) { mine = best; word = low; }
+    if (lane == win) {
+#pragma unroll
+      for (int j = 0; j < M; ++j)
+        if (j == bj) {
+          const int at = ++pos[j], u = lane * M + j;
+          uint2 e = make_uint2(0xff800000u, 0xffffffffu);
+          if (at < S) e = stage[u * S + at];
+          else if (at < K) e = list[(int64_t)u * K + at];
+          hv[j] = __uint_as_float(e.x);
+          hi[j] = e.y;
+        }
+    }
+  }
+  return found;
+}
+
+// One workgroup per group.  A wave per beam joins the sums and merges the units' lists into the beam's `beams` best; then the beams are merged (or compared
+// in pairs).  Bound by its chain of dependent steps -- 7 us for up to 5 beams, 11 for 9, 44 for 32, of which the units' lists take half -- so everything that can be
+// loaded is loaded at once: a row that was not scanned has whatever lay in the workspace, and does not use it.  (Looking through all candidates for every place,
+// and beams^4 pairs, took a call of one group from 15 us with 5 beams to 62 with 12, 119 with 16 and 1114 with 32; now 22, 27 and 56.)
+__global__ __launch_bounds__(1024) void beam_join_kernel(const BeamParams p) {
   __shared__ double total[kBeamMost * kBeamMost];  // of the continuations of all beams: beam * beams + place
   __shared__ double rank[kBeamMost * kBeamMost];
   __shared__ uint32_t token[kBeamMost * kBeamMost];
-  __shared__ int better[kBeamMost * kBeamMost], place[kBeamMost], len[kBeamMost];
+  __shared__ int better[kBeamPairs * kBeamPairs], place[kBeamMost], len[kBeamMost];
   __shared__ bool fin[kBeamMost];
+  __shared__ uint2 stages[16][kBeamStage];
   const int g = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, K = p.beams;
+  uint2* const stage = stages[wave];
+  const int S = p.units * K <= kBeamStage ? K : kBeamStage / p.units;  // (0 for more units than a merge takes)
   for (int b = wave; b < K; b += blockDim.x >> 6) {
     const int row = g * K + b;
-    const int count = p.units * K;
-    const uint2* list = p.unit_top + (int64_t)row * count;
+    const uint2* list = p.unit_top + (int64_t)row * p.units * K;
     const float* um = p.unit_max + (int64_t)row * p.units;
     const double* us = p.unit_sum + (int64_t)row * p.units;
-    // up to four candidates a lane are kept in registers, more are read again for every place
-    const bool few = count <= 256;
-    float cv[4];
-    uint32_t ci[4];
+    uint2 head[kBeamStage / 64];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int c = lane + j * 64;
-      const uint2 e = few && c < count ? list[c] : make_uint2(0xff800000u, 0xffffffffu);
-      cv[j] = __uint_as_float(e.x);
-      ci[j] = e.y;
+    for (int j = 0; j < kBeamStage / 64; ++j) {
+      const int e = lane + j * 64;
+      head[j] = list[e < p.units * S ? (S == K ? e : e / S * K + e % S) : 0];
     }
     const float m0 = lane < p.units ? um[lane] : -INFINITY;
     const double s0 = lane < p.units ? us[lane] : 0.0;
     const bool done = p.finished[row] != 0;
     const double score = (double)p.scores[row];
     const int after = p.lengths[row] + (done ? 0 : 1);
+#pragma unroll
+    for (int j = 0; j < kBeamStage / 64; ++j) stage[lane + j * 64] = head[j];
     double lse = NAN;
     if (!done && score > -INFINITY) {
       float top = m0;
@@ -214,51 +276,46 @@ __global__ __launch_bounds__(512) void beam_join_kernel(const BeamParams p) {
       for (int u = lane + 64; u < p.units; u += 64) sum += um[u] > -INFINITY ? us[u] * exp((double)um[u] - (double)top) : us[u];
       lse = (double)top + log(dpp_sum(sum));
     }
+    double mark = -INFINITY;       // lane k's continuation, k < K: its total and its word
+    uint32_t word = 0xffffffffu;
     if (lse > -INFINITY && lse < INFINITY) {
-      float v0 = INFINITY, mine = -INFINITY;  // the last one taken; lane k's: the k-th
-      uint32_t i0 = 0, word = 0xffffffffu;
+      float mine = -INFINITY;
       int found = 0;
-      for (; found < K; ++found) {
-        float bv = -INFINITY;
-        uint32_t bi = 0xffffffffu;
-        if (few) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (cv[j] > bv || (cv[j] == bv && ci[j] < bi)) { bv = cv[j]; bi = ci[j]; }
-        } else {
-          for (int c = lane; c < count; c += 64) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's stage is in LDS
+      if (p.units <= 64) {
+        found = merge_units<1>(list, stage, p.units, S, K, lane, mine, word);
+      } else if (p.units <= kBeamStage) {
+        found = merge_units<kBeamStage / 64>(list, stage, p.units, S, K, lane, mine, word);
+      } else {                                            // a vocabulary of more than 524288: every place looks through all lists
+        float v0 = INFINITY;
+        uint32_t i0 = 0;
+        for (; found < K; ++found) {
+          float bv = -INFINITY;
+          uint32_t bi = 0xffffffffu;
+          for (int c = lane; c < p.units * K; c += 64) {
             const uint2 e = list[c];
             const float v = __uint_as_float(e.x);
             if ((v < v0 || (v == v0 && e.y > i0)) && (v > bv || (v == bv && e.y < bi))) { bv = v; bi = e.y; }
           }
-        }
-        const float best = dpp_max(bv);
-        if (!(best > -INFINITY)) break;
-        uint32_t low = bv == best ? bi : 0xffffffffu;
-        const unsigned long long who = __ballot(bv == best);
-        if ((who & (who - 1)) == 0) {
-          low = (uint32_t)__builtin_amdgcn_readlane((int)bi, __ffsll(who) - 1);
-        } else {
+          const float best = dpp_max(bv);
+          if (!(best > -INFINITY)) break;
+          uint32_t low = bv == best ? bi : 0xffffffffu;
 #pragma unroll
           for (int o = 32; o > 0; o >>= 1) { const uint32_t y = __shfl_xor(low, o); low = y < low ? y : low; }
+          v0 = best;
+          i0 = low;
+          if (lane == found) { mine = best; word = low; }
         }
-        v0 = best;
-        i0 = low;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (ci[j] == low) { cv[j] = -INFINITY; ci[j] = 0xffffffffu; }
-        if (lane == found) { mine = best; word = low; }
       }
-      if (lane < K) {
-        total[b * K + lane] = lane < found ? score + ((double)mine - lse) : -INFINITY;
-        token[b * K + lane] = word;
-      }
-      if (found < K && lane == 0) {  // all finite ones are listed: the first words that are not, at -inf
+      if (lane < found) mark = score + ((double)mine - lse);
+      if (found < K) {                                    // all finite ones are listed: the first words that are not, at -inf
+        if (lane < found) token[b * K + lane] = word;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         uint32_t t = 0;
-        for (int k = found; k < K; ++k, ++t) {
+        for (int k = found; k < K; ++k, ++t) {            // (every lane alike)
           for (int d = 0; d < found; ++d)
             if (token[b * K + d] == t) { ++t; d = -1; }
-          token[b * K + k] = t < (uint32_t)p.vocab ? t : 0xffffffffu;
+          if (lane == k) word = t < (uint32_t)p.vocab ? t : 0xffffffffu;
         }
       }
     } else if (lane < K) {
@@ -266,30 +323,72 @@ __global__ __launch_bounds__(512) void beam_join_kernel(const BeamParams p) {
       const int eos = (int)p.eos;
       const bool alive = done && score > -INFINITY;
       const int t = !alive ? lane : lane == 0 ? eos : (lane - 1 < eos ? lane - 1 : lane);
-      total[b * K + lane] = alive && lane == 0 ? score : -INFINITY;
-      token[b * K + lane] = t < p.vocab ? (uint32_t)t : 0xffffffffu;
+      if (alive && lane == 0) mark = score;
+      word = t < p.vocab ? (uint32_t)t : 0xffffffffu;
     }
     if (lane < K) {
-      const double base = (double)(after > 1 ? after : 1);
-      const double r = p.penalty == 0.0 ? total[b * K + lane] : total[b * K + lane] / (p.penalty == 1.0 ? base : pow(base, p.penalty));
-      rank[b * K + lane] = r == r ? r : -INFINITY;       // (-inf over a power that overflows; every pair has to have an order)
+      total[b * K + lane] = mark;
+      token[b * K + lane] = word;
     }
-    if (lane < K) better[b * K + lane] = 0;
-    if (lane == 0) place[b] = 0;
     if (lane == 0) { fin[b] = done; len[b] = after; }
   }
   __syncthreads();
-  // every pair of continuations is compared by a thread of its own
-  const int all = K * K;
-  for (int x = tid; x < all * all; x += blockDim.x) {
-    const int c = x / all, d = x - c * all;
-    if (token[d] == 0xffffffffu) continue;               // (a vocabulary smaller than the beams)
-    const double r = rank[c], q = rank[d];
-    if (q > r || (q == r && (d / K < c / K || (d / K == c / K && token[d] < token[c])))) atomicAdd(&better[c], 1);
+  // a thread per continuation: its rank, and its place among its beam's -- a rank may be a tie where the logits were none, and the lower word comes first then
+  const bool mine = tid < K * K;                          // (the workgroup has as many threads)
+  const int first = tid / K * K;                          // of the beam
+  double mark = 0.0, r = 0.0;
+  uint32_t word = 0xffffffffu;
+  if (mine) {
+    mark = total[tid];
+    word = token[tid];
+    const double base = (double)(len[tid / K] > 1 ? len[tid / K] : 1);
+    r = p.penalty == 0.0 ? mark : mark / (p.penalty == 1.0 ? base : pow(base, p.penalty));
+    if (!(r == r)) r = -INFINITY;                         // (-inf over a power that overflows; every pair has to have an order)
+    rank[tid] = r;
+    if (K <= kBeamPairs) better[tid] = 0;
   }
   __syncthreads();
-  for (int c = tid; c < all; c += blockDim.x)
-    if (token[c] != 0xffffffffu && better[c] < K) place[better[c]] = c;
+  if (K <= kBeamPairs) {                                  // every pair of continuations is compared by a thread of its own
+    const int all = K * K;
+    for (int x = tid; x < all * all; x += blockDim.x) {
+      const int c = x / all, d = x - c * all;
+      const double a = rank[c], q = rank[d];
+      if (token[d] != 0xffffffffu && (q > a || (q == a && (d / K < c / K || (d / K == c / K && token[d] < token[c]))))) atomicAdd(&better[c], 1);
+    }
+    __syncthreads();
+    if (mine && word != 0xffffffffu && better[tid] < K) place[better[tid]] = tid;
+  } else {
+    int at = 0;
+    if (mine) {
+#pragma unroll 4
+      for (int d = first; d < first + K; ++d) {
+        const double q = rank[d];
+        const uint32_t y = token[d];                      // none (a vocabulary smaller than the beams): behind the others
+        at += word == 0xffffffffu ? y != word || d < tid : y != 0xffffffffu && (q > r || (q == r && y < word));
+      }
+    }
+    __syncthreads();
+    if (mine) {
+      total[first + at] = mark;
+      rank[first + at] = r;
+      token[first + at] = word;
+    }
+    __syncthreads();
+    if (wave == 0) {                                      // lane b watches beam b; of equal ranks the lowest beam's comes first
+      int c = lane * K;
+      bool some = lane < K && token[c] != 0xffffffffu;
+      double v = some ? rank[c] : -INFINITY;
+      for (int k = 0; k < K; ++k) {
+        const double best = dpp_max(v);
+        const unsigned long long who = __ballot(some && v == best);
+        if (lane == __ffsll(who) - 1) {
+          place[k] = c++;
+          some = c < (lane + 1) * K && token[c] != 0xffffffffu;
+          v = some ? rank[c] : -INFINITY;
+        }
+      }
+    }
+  }
   __syncthreads();
   for (int k = tid; k < K; k += blockDim.x) {
     const int c = place[k], b = c / K, to = g * K + k;
@@ -352,6 +451,6 @@ extern "C" int mmamd_beam_search_step(const void* logits, int dtype, int64_t ld,
   if (dtype == MMAMD_F32) beam_scan_kernel<float><<<grid, 256, lds, st>>>(p);
   else beam_scan_kernel<bf16><<<grid, 256, lds, st>>>(p);
   if (int rc = launch_status("beam_search_step scan")) return rc;
-  beam_join_kernel<<<groups, 64 * (beams < 8 ? beams : 8), 0, st>>>(p);
+  beam_join_kernel<<<groups, 64 * (beams < 8 ? 8 : beams < 16 ? beams : 16), 0, st>>>(p);
   return launch_status("beam_search_step");
 }

@@ -146,3 +146,23 @@ def test_streams_and_graphs():
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, eager))
         check(*live, 11, 0.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("groups,beams,vocab", [(2, 9, 49408), (1, 16, 49408), (1, 31, 49408), (2, 17, 997), (1, 5, 131072), (1, 5, 131073), (1, 12, 200003), (1, 3, 524289), (1, 20, 600011)])
+def test_many_beams_and_words(groups, beams, vocab, dtype):
+    """More beams than waves, more lists than lanes, lists longer than their part in LDS."""
+    check(*make(11, groups, beams, vocab, dtype), vocab // 3, 0.6)
+
+
+@pytest.mark.parametrize("beams,vocab", [(4, 140000), (20, 49408), (32, 600011)])
+def test_the_best_in_one_stretch_and_ties_far_apart(beams, vocab):
+    """All of a row's best words lie beside each other (one list is used up), then all over it at equal logits."""
+    logits, scores, lengths, finished, seq = make(12, 1, beams, vocab, ended=0.0)
+    logits[:, 30000:30000 + beams] += 50.0
+    check(logits, scores, lengths, finished, seq, 9, 1.0)
+    logits[:] = -1.0
+    logits[:, 777::9001] = 2.0
+    logits[:, vocab - 1] = 2.0
+    scores[:] = -0.5 - torch.arange(beams, device="cuda") / 64.0  # (ranks of beams differ by more than a rounding)
+    check(logits, scores, lengths, finished, seq, 9, 0.0)
