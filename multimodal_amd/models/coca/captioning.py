@@ -47,8 +47,8 @@ class _Search:
         self.caches = []
         for decoder in (self.text, self.fusion.transformer_decoder):
             att = decoder.layer[0].attention
-            pages = rows * (-(-max_length // page_size) + 2)
-            self.caches.append(PagedKVCache(len(decoder.layer), att.num_heads, att.q_proj.out_features // att.num_heads, max(1, pages), max_length, page_size, device=dev))
+            pages = PagedKVCache.pages_for(rows, max_length, page_size)
+            self.caches.append(PagedKVCache(len(decoder.layer), att.num_heads, att.q_proj.out_features // att.num_heads, pages, max_length, page_size, device=dev))
         # the beams of an image read the same pages, and a beam is only ever continued within its image: one table for the whole search
         cross = self.fusion.transformer_decoder.cross_cache(states.contiguous(), page_size)
         self.caches[1].cross = cross.shared_rows(torch.arange(bsz, device=dev).repeat_interleave(beams))

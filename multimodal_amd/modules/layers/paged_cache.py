@@ -22,7 +22,8 @@ class PagedKVCache:
         cache.fork(parents, reserve=1)                      # rows of the next token: beams reordered, rows dropped or doubled
         decoder(token_states, past_key_values=cache)        # [rows, 1, d]
 
-    num_pages has to cover what is live and, at a fork, what is fresh beside it: rows * (slots + 2) is always enough.  What could not be had is counted in
+    num_pages has to cover what is live and, at a fork, what is fresh beside it: pages that were reserved and hold no token yet are taken anew by every fork,
+    while the old rows' still count.  pages_for() is always enough, less serves rows that share pages or end early.  What could not be had is counted in
     `shortage` (int32 [1], of the last fork); those tokens are lost."""
 
     def __init__(self, n_layer: int, num_heads: int, head_dim: int, num_pages: int, max_tokens: int, page_size: int = 16, dtype: torch.dtype = torch.bfloat16,
@@ -36,6 +37,15 @@ class PagedKVCache:
         self.cross: Optional["PagedKVCache"] = None  # keys and values of encoder states, for decoders with cross-attention, row for row
         self._view = False
         self.reset()
+
+    @staticmethod
+    def pages_for(rows: int, max_tokens: int, page_size: int = 16, reserve: int = 1) -> int:
+        """Pages that suffice whatever happens, for at most `rows` rows of max_tokens tokens before and after every fork, none of which asks for more than `reserve`
+        tokens a row (nor add_rows, where rows are there already): the old rows' pages, and a fresh row's copy of a partial page and its reserved ones."""
+        if min(rows, max_tokens, page_size) < 1 or reserve < 0:
+            raise ValueError(f"rows, max_tokens and page_size must be at least 1 and reserve at least 0, got {rows}, {max_tokens}, {page_size}, {reserve}")
+        slots = -(-max_tokens // page_size)
+        return rows * (slots + min(slots, 1 - (-reserve // page_size)))
 
     def reset(self) -> None:
         """No rows, every page free."""
