@@ -61,7 +61,7 @@ class _Search:
         self.sequences = torch.full((bsz, beams, max_length - 1), end, dtype=torch.int64, device=dev)  # what follows the begin token
         self.tokens = torch.full((bsz, beams), begin, dtype=torch.int64, device=dev)
         self.place = self.positions[:1].clone()
-        self.held = [[c.page_table, c.lengths, c.refcounts] for c in self.caches]
+        self.held = [[c.page_table, c.lengths, c.refcounts, c.lost] for c in self.caches]
 
     def step(self) -> None:
         """One more token of every beam."""
@@ -73,9 +73,9 @@ class _Search:
             to.copy_(new)
         for cache, held in zip(self.caches, self.held):
             cache.fork(r.parents, reserve=1, cross=False)
-            for to, new in zip(held, (cache.page_table, cache.lengths, cache.refcounts)):
+            for to, new in zip(held, (cache.page_table, cache.lengths, cache.refcounts, cache.lost)):
                 to.copy_(new)
-            cache.page_table, cache.lengths, cache.refcounts = held
+            cache.page_table, cache.lengths, cache.refcounts, cache.lost = held
 
     def run(self, steps: int, graph: bool) -> None:
         replay = None
@@ -99,6 +99,8 @@ class _Search:
                 break
         if replay is not None:
             torch.cuda.current_stream().synchronize()  # the graph's own memory goes with it
+        if int(self.caches[0].lost + self.caches[1].lost) != 0:
+            raise ops.MmamdError("generate_captions: keys and values had no page to go to (PagedKVCache.lost)")
 
 
 @torch.no_grad()

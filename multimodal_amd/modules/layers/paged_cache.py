@@ -24,7 +24,8 @@ class PagedKVCache:
 
     num_pages has to cover what is live and, at a fork, what is fresh beside it: pages that were reserved and hold no token yet are taken anew by every fork,
     while the old rows' still count.  pages_for() is always enough, less serves rows that share pages or end early.  What could not be had is counted in
-    `shortage` (int32 [1], of the last fork); those tokens are lost."""
+    `shortage` (int32 [1], of the last fork) and added to `lost` (int32 [1], since reset()): tokens of those places are gone, the rows' outputs are wrong from there
+    on, and what is done with a search's results should look at `lost` first."""
 
     def __init__(self, n_layer: int, num_heads: int, head_dim: int, num_pages: int, max_tokens: int, page_size: int = 16, dtype: torch.dtype = torch.bfloat16,
                  device: Union[str, torch.device] = "cuda") -> None:
@@ -56,6 +57,7 @@ class PagedKVCache:
         self.lengths = torch.empty((0,), dtype=torch.int32, device=dev)
         self.refcounts = torch.zeros((self.pages.shape[0],), dtype=torch.int32, device=dev)
         self.shortage = torch.zeros((1,), dtype=torch.int32, device=dev)
+        self.lost = torch.zeros((1,), dtype=torch.int32, device=dev)
         self._prompt: Union[None, int, Tensor] = None
 
     @property
@@ -95,6 +97,7 @@ class PagedKVCache:
             follow = self.cross
         s = ops.paged_fork(self.pages, self.page_table, self.lengths, self.refcounts, parents.reshape(-1), reserve=reserve)
         self.page_table, self.lengths, self.refcounts, self.shortage = s
+        self.lost = self.lost + s.shortage
         self.cross = follow
         self._prompt = None
 

@@ -255,3 +255,19 @@ def test_captions_of_two_streams_and_two_threads():
     for t in threads:
         t.join()
     check()
+
+
+@pytest.mark.parametrize("graph", [False, True], ids=["eager", "graph"])
+@torch.no_grad()
+def test_captions_that_lost_keys_are_not_returned(graph, monkeypatch):
+    """A pool that is too small from some step on, also where that step is a replay."""
+    from multimodal_amd import ops
+    from multimodal_amd.models.coca.captioning import generate_captions
+    from multimodal_amd.modules.layers.paged_cache import PagedKVCache
+
+    model = coca(SMALL, False, 63)
+    images = torch.randn(2, 3, 64, 64, generator=torch.Generator().manual_seed(7)).cuda()
+    generate_captions(model, images, 1, 2, num_beams=2, page_size=2, graph=graph)
+    monkeypatch.setattr(PagedKVCache, "pages_for", staticmethod(lambda rows, *a: rows * 3))
+    with pytest.raises(ops.MmamdError, match="lost"):
+        generate_captions(model, images, 1, 2, num_beams=2, page_size=2, graph=graph)

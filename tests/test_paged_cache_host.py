@@ -76,3 +76,20 @@ def test_pages_for_refuses_nonsense():
     for bad in ((0, 4, 4, 1), (2, 0, 4, 1), (2, 4, 0, 1), (2, 4, 4, -1)):
         with pytest.raises(ValueError):
             PagedKVCache.pages_for(*bad)
+
+
+def test_losses_stay_on_record(on_cpu):
+    """A page that could not be had is not forgotten by the next fork, which has nothing to report."""
+    c = cache(5, 32, 4)
+    c.fork(torch.tensor([-1, -1], dtype=torch.int32), reserve=9)
+    assert int(c.shortage) == 1 and int(c.lost) == 1
+    c.advance(9)
+    c.fork(torch.tensor([0], dtype=torch.int32), reserve=0)
+    assert int(c.shortage) == 0 and int(c.lost) == 1
+    c.fork(torch.tensor([0, 0, 0, 0], dtype=torch.int32), reserve=1)  # three copies of the partial page for two free ones
+    assert int(c.shortage) == 1 and int(c.lost) == 2
+    c.reserve(1)
+    assert int(c.shortage) == 0 and int(c.lost) == 2
+    assert c.shared_rows(torch.tensor([0])).lost is c.lost
+    c.reset()
+    assert int(c.lost) == 0
