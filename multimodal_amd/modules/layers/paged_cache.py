@@ -22,10 +22,13 @@ class PagedKVCache:
         cache.fork(parents, reserve=1)                      # rows of the next token: beams reordered, rows dropped or doubled
         decoder(token_states, past_key_values=cache)        # [rows, 1, d]
 
+    A decoder's step takes room for its token by itself where none is left of an int `reserve`; with one per row the room is the caller's.
+
     num_pages has to cover what is live and, at a fork, what is fresh beside it: pages that were reserved and hold no token yet are taken anew by every fork,
     while the old rows' still count.  pages_for() is always enough, less serves rows that share pages or end early.  What could not be had is counted in
-    `shortage` (int32 [1], of the last fork) and added to `lost` (int32 [1], since reset()): tokens of those places are gone, the rows' outputs are wrong from there
-    on, and what is done with a search's results should look at `lost` first."""
+    `shortage` (int32 [1], of the last fork) and added to `lost` (int32 [1], since reset()), and so are tokens beyond a row's table, and those of a decoder's step
+    whose row got no room by a `reserve` per row: tokens of those places are gone, the rows' outputs are wrong from there on, and what is done with a search's results
+    should look at `lost` first.  (Replays of a captured step advance the lengths unseen: where they pass max_tokens is the caller's to know.)"""
 
     def __init__(self, n_layer: int, num_heads: int, head_dim: int, num_pages: int, max_tokens: int, page_size: int = 16, dtype: torch.dtype = torch.bfloat16,
                  device: Union[str, torch.device] = "cuda") -> None:
@@ -59,6 +62,9 @@ class PagedKVCache:
         self.shortage = torch.zeros((1,), dtype=torch.int32, device=dev)
         self.lost = torch.zeros((1,), dtype=torch.int32, device=dev)
         self._prompt: Union[None, int, Tensor] = None
+        # what the host knows without asking the device: tokens that every row has room for (None: of each row's own), and the most that a row may hold (None: unknown)
+        self._room: Optional[int] = 0
+        self._most: Optional[int] = 0
 
     @property
     def rows(self) -> int:
@@ -83,7 +89,7 @@ class PagedKVCache:
         if isinstance(tokens, int) and tokens > room:
             raise ValueError(f"prompts of {tokens} tokens for rows of {room}")
         self.fork(torch.full((rows,), -1, dtype=torch.int32, device=self.pages.device), reserve=tokens, cross=False)
-        self._prompt = tokens
+        self._prompt, self._most = tokens, 0
 
     def fork(self, parents: Tensor, reserve: Union[int, Tensor] = 1, cross: bool = True) -> None:
         """Row r becomes a continuation of the present row parents[r] (int32, any shape, -1: an empty row) with room for `reserve` more tokens.  The rows of
@@ -98,6 +104,7 @@ class PagedKVCache:
         s = ops.paged_fork(self.pages, self.page_table, self.lengths, self.refcounts, parents.reshape(-1), reserve=reserve)
         self.page_table, self.lengths, self.refcounts, self.shortage = s
         self.lost = self.lost + s.shortage
+        self._room = None if isinstance(reserve, Tensor) else int(reserve)
         self.cross = follow
         self._prompt = None
 
@@ -137,10 +144,39 @@ class PagedKVCache:
         return ops.paged_attention(q, kp, vp, self.page_table, self.lengths, k, v, scale)
 
     def advance(self, tokens: Union[int, Tensor] = 1) -> None:
-        """Counts tokens that every layer has stored."""
+        """Counts tokens that every layer has stored.  A length ends at the table's room; what is beyond it has no place and is counted in `lost`."""
         self._owned("advance")
-        self.lengths = self.lengths + tokens
-        self._prompt = None
+        if isinstance(tokens, Tensor):
+            self._advance(tokens, None, None)
+        else:
+            self._advance(tokens, self._most + tokens if self._most is not None else None, max(0, self._room - tokens) if self._room is not None else None)
+
+    def _advance(self, tokens: Union[int, Tensor], most: Optional[int], room: Optional[int]) -> None:
+        cap = self.page_table.shape[1] * self.page_size
+        after = self.lengths + tokens
+        if most is None or most > cap:
+            self.lengths, most = after.clamp(max=cap), cap
+            self.lost = self.lost + (after - self.lengths).sum(dtype=torch.int32)
+        else:
+            self.lengths = after
+        self._prompt, self._most, self._room = None, most, room
+
+    def _stored_prompt(self, tokens: int) -> None:
+        """advance() for the prompts [rows, tokens, ...] that add_rows announced (a count beyond the prompt has stored nothing there)."""
+        if isinstance(self._prompt, Tensor):
+            self._advance(self._prompt.clamp(0, tokens), tokens, 0)
+        else:
+            self.advance(tokens)
+
+    def _make_room(self) -> None:
+        """Before a step: a place for each row's token where the host knows that none was asked for; where it does not know, tokens without one are counted."""
+        if self._room == 0:
+            self.reserve(1)
+        elif self._room is None and self.rows > 0:
+            slots = self.page_table.shape[1]
+            at = torch.div(self.lengths, self.page_size, rounding_mode="floor").long()
+            page = torch.gather(self.page_table, 1, at.clamp(0, slots - 1)[:, None])[:, 0]
+            self.lost = self.lost + ((at < slots) & ((page < 0) | (page >= self.pages.shape[0]))).sum(dtype=torch.int32)
 
     def compact(self) -> int:
         """Moves the live pages to the front and says how many they are (this waits for the device)."""

@@ -552,12 +552,17 @@ def _decoder_forward_paged(self, hidden_states: Tensor, encoder_hidden_states, c
         Sk = encoder_hidden_states.shape[1]
         enc = ops.convert(_f32_rows(encoder_hidden_states, "TransformerDecoder"), torch.bfloat16)
     hidden = []
-    prompt = cache._prompt
+    step = cache._prompt is None
+    if step and S == 1 and B == cache.rows:  # (run_paged refuses other steps)
+        cache._make_room()
     for i, layer_module in enumerate(self.layer):
         if return_hidden_states:
             hidden.append(x.view(B, S, d))
         x = layer_module.run_paged(x, B, S, cache, i, enc, Sk)
-    cache.advance(1 if prompt is None else prompt if isinstance(prompt, int) else prompt.clamp(0, S))  # (a count beyond the prompt has stored nothing there)
+    if step:
+        cache.advance(1)
+    else:
+        cache._stored_prompt(S)
     x = x.view(B, S, d)
     if return_hidden_states:
         hidden.append(x)

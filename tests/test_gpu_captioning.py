@@ -260,7 +260,8 @@ def test_captions_of_two_streams_and_two_threads():
 @pytest.mark.parametrize("graph", [False, True], ids=["eager", "graph"])
 @torch.no_grad()
 def test_captions_that_lost_keys_are_not_returned(graph, monkeypatch):
-    """A pool that is too small from some step on, also where that step is a replay."""
+    """A pool that is too small from some step on, also where that step is a replay: with pages of two tokens and two a row, the fourth step finds at least 6 of the 8
+    live (the rows' last pages and a first one per image) and needs 4."""
     from multimodal_amd import ops
     from multimodal_amd.models.coca.captioning import generate_captions
     from multimodal_amd.modules.layers.paged_cache import PagedKVCache
@@ -268,6 +269,27 @@ def test_captions_that_lost_keys_are_not_returned(graph, monkeypatch):
     model = coca(SMALL, False, 63)
     images = torch.randn(2, 3, 64, 64, generator=torch.Generator().manual_seed(7)).cuda()
     generate_captions(model, images, 1, 2, num_beams=2, page_size=2, graph=graph)
-    monkeypatch.setattr(PagedKVCache, "pages_for", staticmethod(lambda rows, *a: rows * 3))
+    monkeypatch.setattr(PagedKVCache, "pages_for", staticmethod(lambda rows, *a: rows * 2))
     with pytest.raises(ops.MmamdError, match="lost"):
         generate_captions(model, images, 1, 2, num_beams=2, page_size=2, graph=graph)
+
+
+@torch.no_grad()
+def test_steps_without_a_reserve_equal_the_causal_pass():
+    """A prompt that fills its page, then single tokens with no fork or reserve between, up to the table's end and one beyond, which is on record."""
+    from multimodal_amd.modules.layers.transformer import TransformerDecoder
+
+    torch.manual_seed(6)
+    dec = TransformerDecoder(n_layer=2, d_model=128, n_head=2, dim_feedforward=256, activation=torch.nn.GELU, layer_norm_eps=1e-5, norm_first=True,
+                             use_cross_attention=False).cuda().eval()
+    x = torch.randn(2, 13, 128, generator=torch.Generator().manual_seed(8)).cuda()
+    full = dec(x[:, :12], attention_mask=causal(12)).last_hidden_state
+    cache = cache_for(dec, 2, 12, 4)
+    cache.pages.fill_(float("nan"))
+    cache.add_rows(2, 4)
+    got = [dec(x[:, :4], past_key_values=cache).last_hidden_state]
+    got += [dec(x[:, t:t + 1], past_key_values=cache).last_hidden_state for t in range(4, 12)]
+    assert np.abs(host(torch.cat(got, 1)) - host(full)).max() <= 2e-2  # (as in the tests above)
+    assert int(cache.lost) == 0 and host(cache.lengths).tolist() == [12, 12]
+    dec(x[:, 12:], past_key_values=cache)
+    assert int(cache.lost) == 2 and host(cache.lengths).tolist() == [12, 12]

@@ -93,3 +93,116 @@ def test_losses_stay_on_record(on_cpu):
     assert c.shared_rows(torch.tensor([0])).lost is c.lost
     c.reset()
     assert int(c.lost) == 0
+
+
+# ---- the decoder's use of a cache: layers of one linear map, attention by the restatements -------------------------------------------------
+
+
+class _Decoder:
+    """TransformerDecoder._forward_paged without a device: `calls` decoding steps of a one-layer model whose queries, keys and values are its inputs."""
+
+    def __init__(self, monkeypatch):
+        from multimodal_amd.modules.layers import transformer as tr
+
+        class Layer:
+            @staticmethod
+            def run_paged(x, B, S, cache, layer, enc, Sk):
+                rows = x.view(B, S, 1, -1)
+                if S == 1 and cache._prompt is None:
+                    return cache.attend(layer, rows[:, 0], rows[:, 0], rows[:, 0]).reshape(B, -1)
+                cache.append(layer, rows, rows, cache._prompt if isinstance(cache._prompt, torch.Tensor) else None)
+                return x
+
+        monkeypatch.setattr(tr, "wants_grad", lambda m: False)
+        monkeypatch.setattr(tr, "plain_layers", lambda *a: True)
+        monkeypatch.setattr(tr, "_f32_rows", lambda x, who: x.reshape(-1, x.shape[-1]))
+        monkeypatch.setattr(tr, "_check_paged", lambda *a: None, raising=False)
+        self.layer, self.final_layer_norm, self.run = [Layer()], None, tr._decoder_forward_paged
+
+    def __call__(self, x, cache):
+        with torch.no_grad():
+            return self.run(self, x, None, cache, False).last_hidden_state
+
+
+def plain(row):
+    """Attention of the last token of row [n, dim] over all of it."""
+    w = torch.softmax((row.double() @ row[-1].double()) / row.shape[1] ** 0.5, 0)
+    return w @ row.double()
+
+
+def close(out, rows):
+    return all(float((out[r, 0].double() - plain(row)).abs().max()) < 1e-5 for r, row in enumerate(rows))
+
+
+def test_steps_without_a_reserve_are_stored(on_cpu, monkeypatch):
+    """Right behind a prompt that fills its pages, and on and on: every token has its place and is seen."""
+    dec, g = _Decoder(monkeypatch), torch.Generator().manual_seed(0)
+    c = cache(PagedKVCache.pages_for(2, 48), 48)
+    c.add_rows(2, 16)
+    rows = torch.randn(2, 40, 64, generator=g)
+    dec(rows[:, :16], c)
+    for t in range(16, 40):
+        assert close(dec(rows[:, t:t + 1], c), rows[:, :t + 1]), t
+        if t == 30:
+            c.fork(torch.tensor([1, 0], dtype=torch.int32), reserve=0)
+            rows = rows[[1, 0]]
+    assert c.lengths.tolist() == [40, 40] and int(c.lost) == 0
+
+
+def test_reserved_room_is_used_up_before_more_is_asked_for(on_cpu, monkeypatch):
+    dec = _Decoder(monkeypatch)
+    asked = []
+    c = cache(12, 48)
+    c.add_rows(2, 10)
+    x = torch.randn(2, 40, 64, generator=torch.Generator().manual_seed(1))
+    dec(x[:, :10], c)
+    c.reserve(20)
+    real = ops.paged_fork
+    monkeypatch.setattr(ops, "paged_fork", lambda *a, reserve=0: asked.append(reserve) or real(*a, reserve=reserve))
+    for t in range(10, 30):
+        dec(x[:, t:t + 1], c)
+    assert asked == []
+    dec(x[:, 30:31], c)
+    assert asked == [1]
+    c.fork(torch.tensor([0, 1], dtype=torch.int32), reserve=1)
+    dec(x[:, 31:32], c)
+    assert asked == [1, 1]
+
+
+def test_reserves_per_row_are_the_callers_and_what_has_no_place_is_counted(on_cpu, monkeypatch):
+    """With a tensor the host does not know the room: nothing is asked for in its place, and a token that has none is on record."""
+    dec = _Decoder(monkeypatch)
+    c = cache(12, 48)
+    x = torch.randn(2, 40, 64, generator=torch.Generator().manual_seed(2))
+    c.add_rows(2, 16)
+    dec(x[:, :16], c)
+    c.fork(torch.tensor([0, 1], dtype=torch.int32), reserve=torch.tensor([2, 0], dtype=torch.int32))
+    dec(x[:, 16:17], c)
+    assert c.page_table[:, 1].ge(0).tolist() == [True, False] and int(c.lost) == 1
+    dec(x[:, 17:18], c)
+    assert int(c.lost) == 2 and c.lengths.tolist() == [18, 18]
+
+
+def test_tokens_beyond_the_table_are_counted(on_cpu, monkeypatch):
+    """One token past max_tokens, and prompts whose counts are beyond the room: the lengths stay at what is stored, the rest is on record."""
+    dec = _Decoder(monkeypatch)
+    x = torch.randn(2, 40, 64, generator=torch.Generator().manual_seed(3))
+    c = cache(30, 20, 4)
+    c.add_rows(2, torch.tensor([18, 3], dtype=torch.int32))
+    dec(x[:, :18], c)
+    for t in range(18, 23):
+        assert int(c.lost) == max(0, t - 20)
+        c.reserve(1)
+        dec(x[:, t:t + 1], c)
+    assert c.lengths.tolist() == [20, 8] and int(c.lost) == 3
+    for counts, stored, lost in (([25, 7], [20, 7], 5), ([40, -3], [20, 0], 8), ([20, 20], [20, 20], 0)):
+        c = cache(30, 20, 4)
+        c.add_rows(2, torch.tensor(counts, dtype=torch.int32))
+        dec(x[:, :28], c)
+        assert c.lengths.tolist() == stored and int(c.lost) == lost, counts
+    c = cache(30, 20, 4)  # by hand
+    c.add_rows(2, 20)
+    c.append(0, x[:, :20, None], x[:, :20, None])
+    c.advance(20)
+    c.advance(torch.tensor([1, 0], dtype=torch.int32))
+    assert c.lengths.tolist() == [20, 20] and int(c.lost) == 1
