@@ -18,6 +18,7 @@
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/library.h>
 
 #include <cmath>
@@ -492,7 +493,6 @@ struct ArgCheck {
     for (size_t i = 0; same && i < shape.size(); ++i) same = shape[i] < 0 || t.size(i) == shape[i];
     TORCH_CHECK(same, who, ": ", name, " must have the shape ", shape, " (-1: any), got ", t.sizes());
     TORCH_CHECK(t.numel() == 0 || (whole ? t.is_contiguous() : t.size(-1) <= 1 || t.stride(-1) == 1), who, ": ", name, " must be contiguous", whole ? "" : " in its last axis");
-    TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), who, " has no gradient (decoding): call it under torch.no_grad()");
   }
 };
 // an axis of one entry is never stepped along, whatever its stride says
@@ -664,6 +664,70 @@ BeamOut beam_search_step_impl(const Tensor& logits, const Tensor& scores, const 
 }
 BeamOut beam_search_step_meta(const Tensor&, const Tensor& scores, const Tensor&, const Tensor&, const OptTensor& sequences, int64_t, double) { return beam_outputs(scores, sequences); }
 
+// Decoding has no derivatives.  The Autograd kernels refuse what a gradient or a forward-mode tangent would have to pass through (at the call: its outputs are tokens,
+// or states that nothing is trained on), and count what was stored as a change of the tensor, as in-place operations do.  (autogradNotImplementedFallback would
+// box every argument of a call that is as long as its kernel, and takes no operator that both stores and returns.)
+bool has_derivative(const Tensor& t, bool grad, bool tangents) { return (grad && t.requires_grad()) || (tangents && t._fw_grad(0).defined()); }
+bool has_derivative(const OptTensor& t, bool grad, bool tangents) { return t.has_value() && t->defined() && has_derivative(*t, grad, tangents); }
+template <typename... A>
+void no_gradient(const char* who, const A&... tensors) {
+  // (asking for the level once costs less than each tensor's tangent, which a view looks up in its base)
+  const bool grad = at::GradMode::is_enabled(), tangents = torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr;
+  TORCH_CHECK(!((grad || tangents) && (has_derivative(tensors, grad, tangents) || ...)), who, " has no gradient (decoding): call it under torch.no_grad()");
+}
+void changed(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+template <typename F, typename... A>
+auto below_autograd(const c10::TypedOperatorHandle<F>& op, c10::DispatchKeySet keys, const A&... a) { return op.redispatch(keys & c10::after_ADInplaceOrView_keyset, a...); }
+template <typename F>
+c10::TypedOperatorHandle<F> decoding_op(const char* name) { return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>(); }
+
+Tensor paged_attention_autograd(c10::DispatchKeySet ks, const Tensor& q, const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& lengths, const OptTensor& k, const OptTensor& v,
+                                c10::optional<double> scale) {
+  static const auto op = decoding_op<decltype(paged_attention_impl)>("mmamd::paged_attention");
+  no_gradient("paged_attention", q, keys, values, k, v);
+  Tensor out = below_autograd(op, ks, q, keys, values, table, lengths, k, v, scale);
+  if (k.has_value()) { changed(keys); changed(values); }
+  return out;
+}
+void paged_attention_into_autograd(c10::DispatchKeySet ks, const Tensor& q, const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& lengths, const OptTensor& k, const OptTensor& v,
+                                   c10::optional<double> scale, const Tensor& out) {
+  static const auto op = decoding_op<decltype(paged_attention_into)>("mmamd::paged_attention_into");
+  no_gradient("paged_attention", q, keys, values, k, v, out);
+  below_autograd(op, ks, q, keys, values, table, lengths, k, v, scale, out);
+  if (k.has_value()) { changed(keys); changed(values); }
+  changed(out);
+}
+void paged_append_autograd(c10::DispatchKeySet ks, const Tensor& k, const Tensor& v, const Tensor& keys, const Tensor& values, const Tensor& table, const Tensor& start, const OptTensor& counts) {
+  static const auto op = decoding_op<decltype(paged_append_impl)>("mmamd::paged_append");
+  no_gradient("paged_append", k, v, keys, values);
+  below_autograd(op, ks, k, v, keys, values, table, start, counts);
+  changed(keys);
+  changed(values);
+}
+std::tuple<Tensor, Tensor, Tensor, Tensor> paged_fork_autograd(c10::DispatchKeySet ks, const Tensor& pages, const Tensor& table, const Tensor& lengths, const Tensor& refcounts, const Tensor& parents,
+                                                               const OptTensor& reserve_rows, int64_t reserve) {
+  static const auto op = decoding_op<decltype(paged_fork_impl)>("mmamd::paged_fork");
+  no_gradient("paged_fork", pages);
+  auto r = below_autograd(op, ks, pages, table, lengths, refcounts, parents, reserve_rows, reserve);
+  changed(pages);
+  return r;
+}
+std::tuple<Tensor, Tensor, Tensor> paged_compact_autograd(c10::DispatchKeySet ks, const Tensor& pages, const Tensor& table, const Tensor& refcounts) {
+  static const auto op = decoding_op<decltype(paged_compact_impl)>("mmamd::paged_compact");
+  no_gradient("paged_compact", pages);
+  auto r = below_autograd(op, ks, pages, table, refcounts);
+  changed(pages);
+  return r;
+}
+BeamOut beam_search_step_autograd(c10::DispatchKeySet ks, const Tensor& logits, const Tensor& scores, const Tensor& lengths, const Tensor& finished, const OptTensor& sequences, int64_t eos,
+                                  double length_penalty) {
+  static const auto op = decoding_op<decltype(beam_search_step_impl)>("mmamd::beam_search_step");
+  no_gradient("beam_search_step", logits, scores);
+  return below_autograd(op, ks, logits, scores, lengths, finished, sequences, eos, length_penalty);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(mmamd, m) {
@@ -766,4 +830,10 @@ TORCH_LIBRARY_IMPL(mmamd, Autograd, m) {
   for (const char* name : {"packed", "convert", "layernorm", "gemm_bf16", "attn_fwd", "attn_probs", "patch_embed", "embed_tokens", "pool_proj_normalize",
                            "l2_normalize", "activation", "image_embed", "attn_x", "coca_text_embed", "rows_linear_f32", "contrastive_fwd"})
     m.impl(name, torch::autograd::autogradNotImplementedFallback());
+  m.impl("paged_attention", paged_attention_autograd);
+  m.impl("paged_attention_into", paged_attention_into_autograd);
+  m.impl("paged_append", paged_append_autograd);
+  m.impl("paged_fork", paged_fork_autograd);
+  m.impl("paged_compact", paged_compact_autograd);
+  m.impl("beam_search_step", beam_search_step_autograd);
 }
