@@ -10,7 +10,8 @@ from ... import ops
 
 
 class PagedKVCache:
-    """Keys and values of `n_layer` attention layers for a changing set of rows.
+    """Keys and values of `n_layer` attention layers for a changing set of rows.  The decoders serve bfloat16 and 64- or 96-wide heads (prompts of more than 288 tokens: 64);
+    append() and attend() by themselves every type and width of ops.paged_attention.
 
     pages [num_pages, n_layer, 2, num_heads, page_size, head_dim]: a page holds `page_size` tokens of one row for every layer, so that sharing, copying and
     freeing it is one decision.  page_table int32 [rows, slots], lengths int32 [rows], refcounts int32 [num_pages] as in ops.paged_fork; all on the device, and no

@@ -536,6 +536,24 @@ class TransformerDecoder(nn.Module):
         return TransformerOutput(last_hidden_state=x, hidden_states=all_hidden_states, current_key_values=current_key_values)
 
 
+def _check_paged(layers, cache: PagedKVCache, S: int, Sk: int) -> None:
+    """What a pass over a paged cache could not serve, found before any layer stores its keys."""
+    if cache.n_layer != len(layers):
+        raise ValueError(f"the cache has {cache.n_layer} layers, the decoder {len(layers)}")
+    att, cross = layers[0].attention, layers[0].cross_attention  # (the layers of a decoder are alike)
+    for what, held, m in (("the cache", cache, att), ("the encoder states' cache", cache.cross if Sk == 0 else None, cross)):
+        if held is None or m is None:
+            continue
+        dtype, heads, width = held.pages.dtype, held.pages.shape[3], held.pages.shape[5]
+        if dtype != torch.bfloat16 or heads != m.num_heads or width != m.q_proj.out_features // m.num_heads or held.n_layer != len(layers):
+            raise ops.MmamdError(f"{what} holds {held.n_layer} layers of {heads} x {width} in {dtype}, the decoder has {len(layers)} of {m.num_heads} x "
+                                 f"{m.q_proj.out_features // m.num_heads}, served in bfloat16")
+    if S > 288 and att.q_proj.out_features // att.num_heads != 64:
+        raise ops.MmamdError(f"prompts of more than 288 tokens need 64-wide heads, got {S} tokens")
+    if Sk > 288 and cross is not None:
+        raise ops.MmamdError(f"cross-attention over more than 288 encoder states, got {Sk}, is served for single tokens, from a cache (cross_cache)")
+
+
 def _decoder_forward_paged(self, hidden_states: Tensor, encoder_hidden_states, cache: PagedKVCache, return_hidden_states: bool) -> TransformerOutput:
     """Incremental decoding with the keys and values in pages: hidden_states [rows, 1, d] are the rows' next tokens, or [rows, tokens, d] their prompts (after
     PagedKVCache.add_rows).  Every layer stores them, then the cache's lengths are advanced; current_key_values is the cache."""
@@ -543,13 +561,11 @@ def _decoder_forward_paged(self, hidden_states: Tensor, encoder_hidden_states, c
         raise ops.MmamdError("key/value caching is an inference feature: call the decoder under torch.no_grad() / in eval mode")
     if not plain_layers(self.layer, TransformerDecoderLayer):
         raise ops.MmamdError("a paged cache is served by the decoder's own layers only (not wrapped or hooked ones)")
-    if cache.n_layer != len(self.layer):
-        raise ValueError(f"the cache has {cache.n_layer} layers, the decoder {len(self.layer)}")
     B, S, d = hidden_states.shape
+    enc, Sk = None, 0 if encoder_hidden_states is None else encoder_hidden_states.shape[1]
+    _check_paged(self.layer, cache, S, Sk)
     x = _f32_rows(hidden_states, "TransformerDecoder")
-    enc, Sk = None, 0
     if encoder_hidden_states is not None:
-        Sk = encoder_hidden_states.shape[1]
         enc = ops.convert(_f32_rows(encoder_hidden_states, "TransformerDecoder"), torch.bfloat16)
     hidden = []
     step = cache._prompt is None

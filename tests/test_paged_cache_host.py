@@ -206,3 +206,33 @@ def test_tokens_beyond_the_table_are_counted(on_cpu, monkeypatch):
     c.advance(20)
     c.advance(torch.tensor([1, 0], dtype=torch.int32))
     assert c.lengths.tolist() == [20, 20] and int(c.lost) == 1
+
+
+def test_what_a_decoder_cannot_serve_is_refused_before_anything_is_stored():
+    from multimodal_amd.modules.layers.transformer import TransformerDecoder
+
+    def decoder(heads, dim, cross=False):
+        return TransformerDecoder(n_layer=2, d_model=heads * dim, n_head=heads, dim_feedforward=64, use_cross_attention=cross, dim_kv=heads * dim if cross else None).eval()
+
+    def held(heads=2, dim=96, layers=2, dtype=torch.bfloat16):
+        return PagedKVCache(layers, heads, dim, 40, 600, 16, dtype=dtype, device="cpu")
+
+    narrow, wide, crossed = decoder(2, 64), decoder(2, 96), decoder(2, 64, True)
+    x64, x96 = torch.zeros(1, 300, 128), torch.zeros(1, 300, 192)
+    with torch.no_grad():
+        with pytest.raises(ops.MmamdError, match="288 tokens need 64-wide heads, got 300"):
+            wide(x96, past_key_values=held())
+        for c in (held(dtype=torch.float32), held(heads=3), held(dim=128), held(dim=64)):
+            with pytest.raises(ops.MmamdError, match="served in bfloat16"):
+                wide(x96[:, :1], past_key_values=c)
+        with pytest.raises(ValueError, match="3 layers"):
+            wide(x96[:, :1], past_key_values=held(layers=3))
+        c = held(dim=64)
+        with pytest.raises(ops.MmamdError, match="288 encoder states, got 300"):
+            crossed(x64[:, :1], x64, past_key_values=c)
+        c.cross = held(heads=1, dim=128)
+        with pytest.raises(ops.MmamdError, match="the encoder states' cache holds 2 layers of 1 x 128"):
+            crossed(x64[:, :1], past_key_values=c)
+        for dec, x in ((narrow, x64), (wide, x96[:, :288])):  # served; here they end at the first tensor that is not on a device
+            with pytest.raises(Exception, match="CPU|device"):
+                dec(x, past_key_values=held(dim=x.shape[2] // 2))
