@@ -41,6 +41,7 @@ class PagedKVCache:
         self.pages = torch.empty((num_pages, n_layer, 2, num_heads, page_size, head_dim), dtype=dtype, device=device)
         self.cross: Optional["PagedKVCache"] = None  # keys and values of encoder states, for decoders with cross-attention, row for row
         self._view = False
+        self._moves, self._made = [0], 0  # how often pages were moved or taken from under shared_rows() views, which look at their maker's count; its state at their making
         self.reset()
 
     @staticmethod
@@ -55,6 +56,7 @@ class PagedKVCache:
     def reset(self) -> None:
         """No rows, every page free."""
         self._owned("reset")
+        self._moves[0] += 1
         dev = self.pages.device
         slots = -(-self.max_tokens // self.page_size)
         self.page_table = torch.empty((0, slots), dtype=torch.int32, device=dev)
@@ -91,6 +93,7 @@ class PagedKVCache:
             raise ValueError(f"prompts of {tokens} tokens for rows of {room}")
         self.fork(torch.full((rows,), -1, dtype=torch.int32, device=self.pages.device), reserve=tokens, cross=False)
         self._prompt, self._most = tokens, 0
+        self._moves[0] += 1
 
     def fork(self, parents: Tensor, reserve: Union[int, Tensor] = 1, cross: bool = True) -> None:
         """Row r becomes a continuation of the present row parents[r] (int32, any shape, -1: an empty row) with room for `reserve` more tokens.  The rows of
@@ -115,9 +118,12 @@ class PagedKVCache:
 
     def shared_rows(self, parents: Tensor) -> "PagedKVCache":
         """Another view of the same pages: its row r reads what row parents[r] (int64) holds now.  For reading only -- it takes no references, so storing, forking
-        and compacting through it are refused, and this cache has to keep the rows where they are (no fork that drops them, no compact or resize)."""
+        and compacting through it are refused, and this cache has to keep the rows where they are: attending through the view is refused after compact, resize,
+        reset and add_rows; no fork may drop the rows (the host does not see which it drops)."""
         view = object.__new__(PagedKVCache)
         view.__dict__.update(self.__dict__)
+        if not self._view:
+            view._made = self._moves[0]
         view.page_table, view.lengths, view._view = self.page_table[parents], self.lengths[parents], True
         return view
 
@@ -141,6 +147,8 @@ class PagedKVCache:
         """One token a row: q [rows, heads, head_dim] over the row's tokens in `layer`, and over its new one, which is stored, if k and v are given."""
         if k is not None:
             self._owned("attend with new tokens")
+        if self._view and self._made != self._moves[0]:
+            raise ops.MmamdError("attend: the pages of this view's rows were moved or freed by the cache that shared_rows() was called on")
         kp, vp = self.layer(layer)
         return ops.paged_attention(q, kp, vp, self.page_table, self.lengths, k, v, scale)
 
@@ -182,6 +190,7 @@ class PagedKVCache:
     def compact(self) -> int:
         """Moves the live pages to the front and says how many they are (this waits for the device)."""
         self._owned("compact")
+        self._moves[0] += 1
         self.page_table, self.refcounts, live = ops.paged_compact(self.pages, self.page_table, self.refcounts)
         return int(live)
 

@@ -236,3 +236,37 @@ def test_what_a_decoder_cannot_serve_is_refused_before_anything_is_stored():
         for dec, x in ((narrow, x64), (wide, x96[:, :288])):  # served; here they end at the first tensor that is not on a device
             with pytest.raises(Exception, match="CPU|device"):
                 dec(x, past_key_values=held(dim=x.shape[2] // 2))
+
+
+def test_views_of_pages_that_were_moved_are_refused(on_cpu):
+    """compact, resize, reset and add_rows take or move the pages that a shared_rows() view names; a fork that keeps the rows does not."""
+    def fresh():
+        c = cache(20, 32, 4)
+        c.add_rows(3, 5)
+        c.append(0, torch.randn(3, 5, 1, 64), torch.randn(3, 5, 1, 64))
+        c.advance(5)
+        return c, c.shared_rows(torch.tensor([2, 0]))
+
+    q = torch.randn(2, 1, 64)
+    for move in (lambda c: c.compact(), lambda c: c.resize(18), lambda c: c.reset(), lambda c: c.add_rows(2, 3)):
+        c, view = fresh()
+        want = view.attend(0, q)
+        c.reserve(1)
+        assert torch.equal(view.attend(0, q), want)
+        second = view.shared_rows(torch.tensor([1, 0]))
+        move(c)
+        for v in (view, second, view.shared_rows(torch.tensor([0, 1]))):
+            with pytest.raises(ops.MmamdError, match="moved or freed"):
+                v.attend(0, q)
+    c, view = fresh()
+    want = view.attend(0, q)
+    c.compact()
+    assert torch.equal(c.shared_rows(torch.tensor([2, 0])).attend(0, q), want)  # made afterwards, from the same tokens
+    holder, states = cache(20, 32, 4), fresh()[0]
+    holder.cross = states
+    holder.add_rows(3, 1)
+    holder.fork(torch.tensor([2, 2, 0], dtype=torch.int32))
+    holder.cross.attend(0, torch.randn(3, 1, 64))
+    states.resize(19)
+    with pytest.raises(ops.MmamdError, match="moved or freed"):
+        holder.cross.attend(0, torch.randn(3, 1, 64))
