@@ -635,7 +635,10 @@ int mmamd_paged_compact(void* pool, int pages, int64_t page_bytes, const int32_t
 /* One step of a beam search over groups x beams rows of logits [groups * beams, vocab] (fp32 or bf16, row stride ld).  A beam that goes on offers
  * scores[b] + log_softmax(logits[b])[v] for every v, a finished one its own score for v = eos; all others -inf.  The `beams` (<= 32) highest by
  * total / max(length, 1)^length_penalty (finite; length: the continuation's) win, ties go to the lowest b * vocab + v.  A beam with score -inf or NaN, or whose
- * logits have no finite log-sum-exp (a NaN or +inf among them, or nothing but -inf), offers -inf throughout.
+ * logits have no finite log-sum-exp (a NaN or +inf among them, or nothing but -inf), offers -inf throughout; scores are below +inf.
+ * How exact that is: of each beam its `beams` highest logits take part (of equal ones the lowest v), so the order within a beam is exact.  Totals and ranks are
+ * computed in 64 bits, from log-sum-exps of 32-bit exponentials, the 32 of a lane added in 32 bits: good to 5e-8 as a rule and to 2^-18 if every rounding
+ * went one way.  Continuations of different beams that lie nearer to each other than that may change places.
  * lengths int32, finished uint8, sequences int64 [groups, beams, tokens] (NULL: not kept) are reordered: outputs [groups, beams] each, out_parents the row
  * (group * beams + beam) that is continued -- paged_fork's `parents` --, out_sequences with the new token at the parent's length (dropped if there is no
  * room; nothing is added to a finished beam).  Outputs must not overlap inputs. */

@@ -6,7 +6,9 @@
 //
 // Within a beam the order of the totals is the order of the logits, so the vocabulary is read once: every wave takes a stretch of a row and gives its
 // maximum, its sum of exponentials and its `beams` highest logits; a second kernel joins the sums (in 64 bits) and ranks the few that are left, in 64
-// bits as well, since two continuations may lie as near to each other as a rounding to 32.
+// bits as well, so that what lies within a rounding to 32 keeps its order within a beam.  Across beams the log-sum-exps decide: the exponentials
+// are 32-bit ones and a lane adds its 32 in 32 bits, which the scan has time for beside its loads.  That is good to 5e-8 as a rule; at worst 31 additions lose 31 2^-24
+// and the rounding of an exponent (logit - top) log2 e of up to 17 bits 27 2^-24 of the sum, 2^-18 in all.
 #include "common.h"
 
 namespace mmamd {
@@ -87,7 +89,7 @@ __device__ __forceinline__ void beam_load4(const T* p, bool vec, int left, float
 }
 
 // grid: ceil(units / 4) x rows, one unit a wave.  Of the lanes' maxima the `beams`-th highest is a bound that the unit's `beams` best do not fall below:
-// what lies above it (31 values for each of fewer than `beams` lanes, at most, a handful as a rule) and the first of its equals are gathered in LDS,
+// what lies above it (32 values for each of fewer than `beams` lanes, at most, a handful as a rule) and the first of its equals are gathered in LDS,
 // where each counts how many are better.  (Taking the best `beams` times over all 32 values of a lane was bound by its compares and shuffles: 39 us for
 // 512 rows of 49408, 12 us for 5; this way 18 and 6.)  Bound by HBM: 101 MB in 18 us, 5.6 TB/s.
 template <typename T>

@@ -1547,7 +1547,8 @@ def beam_search_step(logits: torch.Tensor, scores: torch.Tensor, lengths: torch.
 
     logits [groups * beams, vocab] fp32 or bf16 (any row stride); scores fp32, lengths int32, finished bool [groups, beams]; sequences int64 [groups, beams,
     tokens] or None.  A beam that goes on offers scores + log_softmax(logits), a finished one only itself (as token `eos`).  The best by
-    total / max(length, 1) ** length_penalty win, ties go to the lowest beam * vocab + token; ranked in 64 bits.  A search begins with scores 0 for the
+    total / max(length, 1) ** length_penalty win, ties go to the lowest beam * vocab + token.  Of each beam its `beams` highest logits take part; ranks are computed in 64 bits
+    from log-sum-exps good to 5e-8 as a rule and 2^-18 at worst, so that continuations of different beams that lie nearer to each other than that may change places.  A search begins with scores 0 for the
     first beam of a group and -inf for the others.  parents is what paged_fork takes (flattened)."""
     try:
         r = _decoding()["beam_search_step"](logits, scores, lengths, finished, sequences, eos, length_penalty)

@@ -166,3 +166,38 @@ def test_the_best_in_one_stretch_and_ties_far_apart(beams, vocab):
     logits[:, vocab - 1] = 2.0
     scores[:] = -0.5 - torch.arange(beams, device="cuda") / 64.0  # (ranks of beams differ by more than a rounding)
     check(logits, scores, lengths, finished, seq, 9, 0.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["fp32", "bf16"])
+@pytest.mark.parametrize("beams,vocab", [(2, 101), (4, 49408), (9, 30522)])
+def test_beams_whose_logits_are_permutations(beams, vocab, dtype):
+    """Equal totals across beams in exact arithmetic: the log-sum-exps, each good to 2^-21 for random logits, decide, so each place holds a continuation within two of those of the exact
+    one; within a beam the order is that of the logits, whatever the sums are."""
+    g = torch.Generator().manual_seed(beams)
+    base = (torch.randn(vocab, generator=g) * 2.5).to(dtype)
+    logits = torch.stack([base[torch.randperm(vocab, generator=g)] for _ in range(2 * beams)]).cuda()
+    scores, done = torch.full((2, beams), -3.25).cuda(), torch.zeros((2, beams), dtype=torch.bool).cuda()
+    got = ops.beam_search_step(logits, scores, torch.full((2, beams), 6, dtype=torch.int32).cuda(), done, None, 3, length_penalty=0.0)
+    logp = torch.log_softmax(logits.cpu().double(), -1)
+    parents, tokens = host(got.parents), host(got.tokens)
+    for k in range(2):
+        best = torch.sort((logp[k * beams:(k + 1) * beams] - 3.25).flatten(), descending=True).values[:beams].numpy()
+        picked = np.array([float(logp[p, t]) - 3.25 for p, t in zip(parents[k], tokens[k])])
+        assert (np.abs(picked - best) <= 2 * 2.0 ** -21).all()
+        assert (np.abs(host(got.scores)[k] - picked) <= 2.0 ** -24 * np.abs(picked) + 2.0 ** -21).all()
+        assert len({(p, t) for p, t in zip(parents[k], tokens[k])}) == beams
+        for b in range(beams):
+            mine = tokens[k][parents[k] == k * beams + b]
+            order = np.lexsort((np.arange(vocab), -logits[k * beams + b].cpu().double().numpy()))
+            np.testing.assert_array_equal(mine, order[:len(mine)])
+
+
+@pytest.mark.parametrize("score", [torch.finfo(torch.float32).min, -1e30])
+def test_scores_that_swallow_the_logits(score):
+    """Ranks that round to one number: of each beam its highest logits take part, and of those the lowest beam's lowest words come first."""
+    logits, scores, lengths, finished, seq = make(9, 2, 5, 5003, ended=0.0)
+    scores.fill_(score)
+    got = ops.beam_search_step(logits, scores, lengths, finished, seq, 0, length_penalty=1.0)
+    best = torch.topk(logits.view(2, 5, -1)[:, 0], 5).indices.sort(1).values
+    assert torch.equal(got.tokens, best) and host(got.parents).tolist() == [[0] * 5, [5] * 5]
+    assert (host(got.scores) == np.float32(score)).all()
