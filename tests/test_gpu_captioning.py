@@ -293,3 +293,92 @@ def test_steps_without_a_reserve_equal_the_causal_pass():
     assert int(cache.lost) == 0 and host(cache.lengths).tolist() == [12, 12]
     dec(x[:, 12:], past_key_values=cache)
     assert int(cache.lost) == 2 and host(cache.lengths).tolist() == [12, 12]
+
+
+class RoundedOtherwise:
+    """multimodal_amd.ops with attention outputs that are moved by up to one step of bf16, at random."""
+
+    def __init__(self, seed_v):
+        from multimodal_amd import ops
+
+        self.ops, self.g = ops, torch.Generator(device="cuda").manual_seed(seed_v)
+
+    def __getattr__(self, name):
+        return getattr(self.ops, name)
+
+    def _moved(self, att):
+        return (att.float() * (1 + 2.0 ** -8 * (2 * torch.rand(att.shape, generator=self.g, device="cuda") - 1))).bfloat16()
+
+    def attention_fwd(self, *args, **kw):
+        return self._moved(self.ops.attention_fwd(*args, **kw))
+
+    def attention_x_fwd(self, *args, **kw):
+        att, probs = self.ops.attention_x_fwd(*args, **kw)
+        return self._moved(att), probs
+
+
+@pytest.mark.parametrize("penalty", [0.0, 1.0])
+@pytest.mark.parametrize("cfg,cascaded", [(SMALL, False), (SMALL, True), (POOL96, False)], ids=["parallel", "cascaded", "three-heads"])
+@torch.no_grad()
+def test_every_step_of_a_search_selects_what_full_forwards_select(cfg, cascaded, penalty, monkeypatch):
+    """Step by step: the model's own full forward over every beam's tokens gives all continuations in 64 bits; the search's beams have to be among the best of them, no two
+    alike, with their totals.
+
+    How far two right log-probabilities of a word may lie apart: the two ways differ in how attention weights and attention outputs are rounded to bf16, by at most half a
+    step, 2^-9 of each, in either way, and in what follows from that.  So the outputs of all the decoders' attentions are moved by up to 2^-8 at random, and twice what that
+    does at most to the log-probabilities of random words is the tolerance."""
+    from multimodal_amd.models.coca import captioning
+    from multimodal_amd.modules.layers import multi_head_attention as mha
+
+    model, bsz, beams, steps, end = coca(cfg, cascaded, 64), 8, 4, 11, 2
+    g = torch.Generator().manual_seed(9)
+    images = torch.randn(bsz, 3, 64, 64, generator=g).cuda()
+    words = torch.randint(3, 96, (bsz, 12), generator=g).cuda()
+    words[:, 0] = 1
+    full = full_log_probs(model, images, words)
+    with monkeypatch.context() as m:
+        m.setattr(mha, "ops", RoundedOtherwise(3))
+        tol = 2 * max(float((full - full_log_probs(model, images, words)).abs().max()) for _ in range(3))
+    assert tol > 0
+    swapped = words.clone()
+    swapped[:, [3, 4]] = words[:, [4, 3]]
+    shown = float((full_log_probs(model, images, swapped) - full)[:, 6:].abs().amax((1, 2)).min())
+    print(f"tolerance {tol:.4f}, two cached words in each other's place change {shown:.4f}")
+    assert shown > 4 * tol
+
+    s = captioning._Search(model, captioning.captioning_embeddings(model, images), 1, end, beams, 12, penalty, 4)
+    state = lambda: [t.clone().cpu().numpy() for t in (s.scores.double(), s.lengths, s.finished, s.sequences)]  # noqa: E731
+    for t in range(steps):
+        scores, lengths, finished, seqs = state()
+        s.place.copy_(s.positions[t:t + 1])
+        s.step()
+        scores2, lengths2, finished2, seqs2 = state()
+        rows = torch.cat([torch.ones(bsz, beams, 1, dtype=torch.int64), torch.from_numpy(seqs[:, :, :t])], 2).cuda()
+        logp = torch.stack([full_log_probs(model, images, rows[:, k].contiguous())[:, t] for k in range(beams)], 1).cpu().numpy()
+        total = scores[..., None] + logp
+        total[finished] = -np.inf
+        total[finished, end] = scores[finished]
+        after = lengths + ~finished
+        rank = total / np.maximum(after, 1)[..., None] ** penalty
+        least = np.sort(rank.reshape(bsz, -1), 1)[:, -beams]
+        for b in range(bsz):
+            taken = set()
+            for k in range(beams):
+                for p in range(beams):  # the beam that it continues: its tokens, and its word
+                    if finished[b, p]:
+                        fits, word = (seqs2[b, k] == seqs[b, p]).all(), end
+                    else:
+                        fits, word = (seqs2[b, k, :t] == seqs[b, p, :t]).all() and scores[b, p] > -np.inf, seqs2[b, k, t]
+                    if fits and lengths2[b, k] == after[b, p] and (p, word) not in taken:
+                        break
+                else:
+                    raise AssertionError((t, b, k, seqs2[b, k], seqs[b]))
+                taken.add((p, word))
+                assert abs(scores2[b, k] - total[b, p, word]) <= (0 if finished[b, p] else tol), (t, b, k)
+                assert rank[b, p, word] >= least[b] - 2 * tol / max(1, after[b, p]) ** penalty, (t, b, k)
+                assert finished2[b, k] == (finished[b, p] or word == end)
+                assert (seqs2[b, k, after[b, p]:] == end).all()
+            place = scores2[b] / np.maximum(lengths2[b], 1) ** penalty
+            assert (np.diff(place) <= 1e-6).all()
+    got = captioning.generate_captions(model, images, 1, end, num_beams=beams, length_penalty=penalty, page_size=4)
+    assert torch.equal(got.sequences[:, :, 1:], s.sequences) and torch.equal(got.scores, s.scores) and torch.equal(got.lengths, s.lengths)
