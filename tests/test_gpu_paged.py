@@ -404,3 +404,40 @@ def test_together():
         state = state._replace(lengths=state.lengths + 1)
     used = host(state.page_table)
     np.testing.assert_array_equal(np.bincount(used[used >= 0].ravel(), minlength=pages), host(state.refcounts))
+
+
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+@torch.no_grad()
+def test_traced_by_torch_compile(backend):
+    """A decoding step in one graph: the operators store through views of one pool, which a graph without in-place operations (aot_eager) has to keep in order."""
+    from multimodal_amd import _torch_ops
+
+    ns = _torch_ops.load()
+
+    def state():
+        g = torch.Generator().manual_seed(4)
+        pool = torch.randn(9, 3, 2, 2, 16, 64, generator=g).to(BF16).cuda()
+        return pool, i32([[0, 1], [2, 3], [4, 5]]), i32([3, 16, 20]), i32([1] * 6 + [0] * 3), i32([2, 2, 0]), torch.randn(3, 8, 64, generator=g).to(BF16).cuda()
+
+    def step(pool, table, lengths, refs, parents, qkv):
+        x, k, v = qkv[:, :4], qkv[:, 4:6], qkv[:, 6:]
+        table, lengths, refs, short = ns.paged_fork(pool, table, lengths, refs, parents, None, 1)
+        for layer in range(3):
+            x = x + ns.paged_attention(x, pool[:, layer, 0], pool[:, layer, 1], table, lengths, k, v, None)
+        ns.paged_append(k[:, None], v[:, None], pool[:, 1, 0], pool[:, 1, 1], table, lengths + 1, None)
+        table, refs, live = ns.paged_compact(pool, table, refs)
+        y = torch.empty_like(x)
+        ns.paged_attention_into(x, pool[:, 1, 0], pool[:, 1, 1], table, lengths + 2, None, None, None, y)
+        best = ns.beam_search_step(y.flatten(1).float(), torch.zeros(1, 3, device="cuda"), lengths[None], lengths[None] < 0, None, 5, 0.0)
+        return (x, y, table, refs, live, short, *best[:5])
+
+    args = state()
+    want, pool = step(*args), args[0]
+    torch._dynamo.reset()
+    compiled = torch.compile(step, backend=backend, fullgraph=True)
+    for _ in range(2):
+        args = state()
+        for a, b in zip(compiled(*args), want):
+            assert torch.equal(a, b)
+        assert torch.equal(args[0], pool)
+    torch._dynamo.reset()
