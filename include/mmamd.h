@@ -602,7 +602,7 @@ typedef struct {
  * q [rows, heads, dim], out the same, contiguous; dtype as the pages.  With k and v ([rows, kv_heads, dim]) the row's new token is first stored at
  * position lengths[r] and t runs over 0 .. lengths[r]; without, over 0 .. lengths[r] - 1.  A row with nothing visible (length 0 without k, negative
  * lengths, no mapped page) gives zeros; a new token that has no place (lengths[r] negative or at the table's end, or its page not mapped) is neither
- * stored nor seen.  Two rows must not have their new tokens in one place.  Softmax statistics and sums in fp32.
+ * stored nor seen.  Two rows must not have their new tokens in one place, nor a token its key and its value; out must not overlap the other arguments.  Softmax statistics and sums in fp32.
  * Workspace: mmamd_paged_attention_workspace bytes (0 where the rows fill the chip by themselves), 16-byte aligned, one per call in flight. */
 int64_t mmamd_paged_attention_workspace(const mmamd_paged_cache* cache, int rows, int heads);
 int mmamd_paged_attention(const mmamd_paged_cache* cache, const int32_t* lengths, const void* q, int64_t q_row, int64_t q_head, const void* k,
@@ -614,7 +614,7 @@ int mmamd_paged_append(const mmamd_paged_cache* cache, const void* k, int64_t k_
                        int64_t v_token, int64_t v_head, const int32_t* start, const int32_t* counts, int rows, int tokens, mmamd_stream_t stream);
 
 /* The pages of a cache.  pool: [pages, blocks, page_size, row_bytes], contiguous (blocks: layers, keys / values, heads); refcounts int32 [pages]: in how
- * many table entries a page stands, free where not positive.
+ * many table entries a page stands, free at 0.  (A negative count is taken for free too, but every entry only adds 1 to it: callers keep counts at 0 or above.)
  * paged_fork builds the tables of `rows` new rows from the old ones: new row r continues old row parents[r] (-1, or any number outside: an empty
  * row).  It shares the parent's full pages.  The partial last page goes to the parent's first child if no other row holds it, all others get a fresh
  * page with a copy of its tokens.  Then fresh pages follow up to reserve_rows[r] (NULL: `reserve`) more tokens.  Entries behind are -1, pages of the

@@ -91,7 +91,7 @@ __device__ __forceinline__ void beam_load4(const T* p, bool vec, int left, float
 // grid: ceil(units / 4) x rows, one unit a wave.  Of the lanes' maxima the `beams`-th highest is a bound that the unit's `beams` best do not fall below:
 // what lies above it (32 values for each of fewer than `beams` lanes, at most, a handful as a rule) and the first of its equals are gathered in LDS,
 // where each counts how many are better.  (Taking the best `beams` times over all 32 values of a lane was bound by its compares and shuffles: 39 us for
-// 512 rows of 49408, 12 us for 5; this way 18 and 6.)  Bound by HBM: 101 MB in 18 us, 5.6 TB/s.
+// 512 rows of 49408, 12 us for 5; this way 19 and 6.)  Bound by HBM: 101 MB in 19 us, 5.3 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void beam_scan_kernel(const BeamParams p) {
   extern __shared__ uint2 lists[];

@@ -70,14 +70,15 @@ __device__ __forceinline__ float across_quarters_max(float v) {
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
 
-// One workgroup: up to 16 query heads of one key head of one row over one split of the row's tokens, so that the cache is read once whatever the group
-// is.  The four waves take the split's tiles (32 tokens in bf16, 16 in fp32) in turn, each with its own running maximum, sum and output:
+// One workgroup: up to 16 query heads of one key head of one row over one split of the row's tokens, so that the cache is requested once for every 16 query heads
+// of a key head (a group of 33: three times), and once for every row that reads a page (beams that share an image's states: 32 x 5 rows over 256 tokens, 12 x 64,
+// request 126 MB of 25 MB, 14.0 us a call).  The four waves take the split's tiles (32 tokens in bf16, 16 in fp32) in turn, each with its own running maximum, sum and output:
 //   scores [token, head] = K . q: the tile's keys go from memory to the registers of a 16 x 16 product as they lie (lane = token, 4 lanes share a row);
 //   out [dim, head] += V^T . weights: the values go through LDS for their columns, the weights are where the first product left them.
 // A pass over a tile ends with the loads of the next one in flight, and the page numbers of the one after.  fp32 runs on the fp32 matrix instruction.
 // bf16 weights are used as two bf16 parts (2^-18 of a weight is lost): in one part they would lose as much as the output's own rounding.
 // Measured, us a call and TB/s of the keys and values: 4 rows of 65536 tokens, 8 x 128, 4 query heads each: 166, 6.5 (a large copy: 4.9); 61 rows of 0 .. 8192
-// tokens, 12 x 64: 67, 4.8 -- what is missing are the first loads of each workgroup and the join; one row of 40 tokens: 4.2, latency.  Two waves a SIMD
+// tokens, 12 x 64: 67, 4.8 -- what is missing are the first loads of each workgroup and the join; one row of 40 tokens: 5.0 (4.2 in a graph), latency.  Two waves a SIMD
 // are enough (with 96 and 128 wide heads; bounds of three or four spill there: 308 and 453 us on the first of these).
 // GROUPS: 16 tokens that begin at a multiple of 16 lie in one page (the page size is a multiple of 16), so their addresses are one scalar and a
 // constant lane offset; otherwise every lane finds the page of one token and the others' come by shuffles.
@@ -434,8 +435,9 @@ static int paged_splits(const mmamd_paged_cache* c, int rows, int heads) {
   return paged_splits((int64_t)rows * c->kv_heads * sub, (int64_t)c->slots * c->page_size, c->dim * (c->dtype == MMAMD_F32 ? 4 : 2));
 }
 
-// A pool of this size or less is read through the caches as usual, a larger one past them.  Us a call, as usual / past them: 1.07 GB 196.6 / 181.1; 322 MB
-// 69.6 / 70.4; 50 MB whose pages eight rows share 110 / 121.
+// A pool of this size or less is read through the caches as usual, a larger one past them: two of the 256 MB that the last cache holds, since a decoder reads its pool
+// again and again, and rows that share pages read them from there.  Us a call, as usual / past them: 1.07 GB 188 / 166; 322 MB, none of it cached, 66.5 / 62.9; 50 MB
+// whose pages eight rows share 33 / 50; 25 MB shared by five 14.0 / 18.3.
 constexpr int64_t kStreamBytes = 512ll << 20;
 
 template <typename T, int D>

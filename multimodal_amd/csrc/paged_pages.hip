@@ -66,7 +66,7 @@ __device__ __forceinline__ int block_scan(int v, int* lds, int& total) {
 
 // Workgroup 0 plans: the lowest child of every parent, the pages each new row needs (numbered over the rows in order), the lowest free pages, the
 // copies.  The others copy the counts, which paged_fork_apply_kernel then changes by what the tables gain and lose.  Bound by its chain of dependent loads:
-// 5.2 us for 160 rows and 965 pages, 7.4 for 384 rows and 10373 pages.
+// 5.6 us for 160 rows and 965 pages, 7.5 for 384 rows and 10373 pages.
 constexpr int kForkOld = 4096;  // old rows whose children are counted in LDS
 __global__ __launch_bounds__(1024) void paged_fork_plan_kernel(const ForkParams p) {
   const int tid = threadIdx.x;
@@ -154,7 +154,7 @@ __global__ __launch_bounds__(1024) void paged_fork_plan_kernel(const ForkParams 
 }
 
 // 1024 16-byte pieces of a copy by one workgroup: four loads a thread in flight, then the stores.  at(i): where piece i lies within a page.  OLD: nobody
-// has touched the source lately, it is read past the caches as well (a large compaction 219 us against 228; a fork's pages were just written: 65 us
+// has touched the source lately, it is read past the caches as well (us a call: a large compaction 219 against 228; a fork's pages were just written: 65
 // against 49).
 template <bool OLD, typename At>
 __device__ __forceinline__ void copy_pieces(const char* from, char* to, uint32_t first, uint32_t end, At at) {
@@ -174,7 +174,7 @@ __device__ __forceinline__ void copy_pieces(const char* from, char* to, uint32_t
 
 // The first rows * share workgroups move data, `share` of them a copy, which split its pieces evenly: the copies differ in their tokens, so cut into stretches of
 // one length they were mostly empty or a second round.  The others write tables: one wave per new row, and one per old row that takes back its references.
-// Bound by HBM: 240 MB in 41 us behind the plan; 53 MB in 7.2 us where they fit the last cache.
+// Bound by HBM: 240 MB in 40.7 us behind the plan, 5.9 TB/s; 53 MB in 9.2 us.
 __global__ __launch_bounds__(256) void paged_fork_apply_kernel(const ForkParams p, uint32_t share, FastDiv per_copy) {
   const uint32_t copiers = (uint32_t)p.rows * share;
   if (blockIdx.x < copiers) {
@@ -302,7 +302,7 @@ __global__ __launch_bounds__(1024) void paged_compact_plan_kernel(const CompactP
 }
 
 // The first `copiers` workgroups walk the moved pages in stretches of 1024 pieces, the others rewrite the table and the counts.  Bound by HBM: 1.14 GB in 210 us,
-// 5.4 TB/s (a large copy: 4.9); 37 MB in 7.2 us.
+// 5.4 TB/s (a large copy: 4.9); 37 MB in 8.2 us.
 __global__ __launch_bounds__(256) void paged_compact_apply_kernel(const CompactParams p, uint32_t pieces, uint32_t stretches, FastDiv per_page, uint32_t copiers) {
   if (blockIdx.x < copiers) {
     uint32_t k = div_by(per_page, blockIdx.x);

@@ -1469,7 +1469,7 @@ def paged_attention(q: torch.Tensor, key_pages: torch.Tensor, value_pages: torch
     for all), heads a multiple of kv_heads; page_table int32 [rows, slots]; lengths int32 [rows] = tokens a row has in the cache.  With k, v [rows, kv_heads,
     dim] the new token is stored at position lengths[row] and seen; lengths are the caller's to advance.  Page numbers outside the pool hold no
     tokens; a row that sees nothing gives zeros.  Places that hold no token may hold anything; an infinite or NaN value of a token makes the outputs it reaches NaN.  scale: 1 / sqrt(dim) unless given.  Two rows' new tokens must not share a place.  out: a contiguous
-    tensor for the result.  All tensors on one device, on whose current stream the work is put."""
+    tensor for the result, apart from the other arguments' memory.  All tensors on one device, on whose current stream the work is put."""
     try:
         if out is None:
             return _decoding()["paged_attention"](q, key_pages, value_pages, page_table, lengths, k, v, scale)
@@ -1512,7 +1512,7 @@ def paged_fork(pages: torch.Tensor, page_table: torch.Tensor, lengths: torch.Ten
     int, or int32 [rows]).  Old rows that nobody continues are thereby freed, and rows can be added.
 
     pages: the whole pool [pages, ..., page_size, dim], contiguous (every layer's keys and values of a page together, so that one call serves them all);
-    page_table int32 [old rows, slots], lengths int32 [old rows], refcounts int32 [pages] = table entries a page stands in (not positive: free).  Fresh
+    page_table int32 [old rows, slots], lengths int32 [old rows], refcounts int32 [pages] = table entries a page stands in (0: free; never below).  Fresh
     pages are the lowest free ones, in the order of the new entries.  Only the copied pages are written, the old state stays as it was."""
     per_row = isinstance(reserve, torch.Tensor)
     try:
