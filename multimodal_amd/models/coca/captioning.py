@@ -73,9 +73,7 @@ class _Search:
             to.copy_(new)
         for cache, held in zip(self.caches, self.held):
             cache.fork(r.parents, reserve=1, cross=False)
-            for to, new in zip(held, (cache.page_table, cache.lengths, cache.refcounts, cache.lost)):
-                to.copy_(new)
-            cache.page_table, cache.lengths, cache.refcounts, cache.lost = held
+            cache._held_in(held)
 
     def run(self, steps: int, graph: bool) -> None:
         replay = None

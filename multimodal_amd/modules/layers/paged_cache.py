@@ -1,7 +1,7 @@
 """Key-value cache in pages for serving the decoders (TransformerDecoder, MultiHeadAttentionWithCache): rows (sequences) are continued, forked, dropped and
 added without moving their keys and values, where the reference concatenates the whole cache per token and layer
 (modules/layers/multi_head_attention.py:158-179) and cannot reorder it.  The operators underneath: ops.paged_attention, paged_append, paged_fork, paged_compact."""
-from typing import Optional, Tuple, Union
+from typing import List, Optional, Tuple, Union
 
 import torch
 from torch import Tensor
@@ -68,6 +68,7 @@ class PagedKVCache:
         # what the host knows without asking the device: tokens that every row has room for (None: of each row's own), and the most that a row may hold (None: unknown)
         self._room: Optional[int] = 0
         self._most: Optional[int] = 0
+        self._room_of = self.page_table  # the table that _room speaks of: one that was put in its place by hand has the room that its maker knows
 
     @property
     def rows(self) -> int:
@@ -108,7 +109,7 @@ class PagedKVCache:
         s = ops.paged_fork(self.pages, self.page_table, self.lengths, self.refcounts, parents.reshape(-1), reserve=reserve)
         self.page_table, self.lengths, self.refcounts, self.shortage = s
         self.lost = self.lost + s.shortage
-        self._room = None if isinstance(reserve, Tensor) else int(reserve)
+        self._room, self._room_of = None if isinstance(reserve, Tensor) else int(reserve), self.page_table
         self.cross = follow
         self._prompt = None
 
@@ -136,6 +137,19 @@ class PagedKVCache:
         view = self.shared_rows(parents.clamp(0, self.rows - 1).long())
         view.lengths = torch.where((parents >= 0) & (parents < self.rows), view.lengths, 0)
         return view
+
+    def _held_in(self, held: List[Tensor]) -> None:
+        """The state moves into tensors that stay where they are: what a captured step reads and what it leaves for its next replay."""
+        for to, new in zip(held, (self.page_table, self.lengths, self.refcounts, self.lost)):
+            to.copy_(new)
+        self._same_room(held[0])
+        self.lengths, self.refcounts, self.lost = held[1:]
+
+    def _same_room(self, table: Tensor) -> None:
+        """`table` takes the present one's place, with as much room in its rows."""
+        if self.page_table is self._room_of:
+            self._room_of = table
+        self.page_table = table
 
     def append(self, layer: int, k: Tensor, v: Tensor, counts: Optional[Tensor] = None) -> None:
         """Stores k, v [rows, tokens, num_heads, head_dim] (counts int32 [rows]: the first ones of each row) behind the rows' tokens; advance() is the caller's."""
@@ -179,9 +193,10 @@ class PagedKVCache:
 
     def _make_room(self) -> None:
         """Before a step: a place for each row's token where the host knows that none was asked for; where it does not know, tokens without one are counted."""
-        if self._room == 0:
+        known = self._room is not None and self.page_table is self._room_of
+        if known and self._room == 0:
             self.reserve(1)
-        elif self._room is None and self.rows > 0:
+        elif not known and self.rows > 0:
             slots = self.page_table.shape[1]
             at = torch.div(self.lengths, self.page_size, rounding_mode="floor").long()
             page = torch.gather(self.page_table, 1, at.clamp(0, slots - 1)[:, None])[:, 0]
@@ -191,7 +206,8 @@ class PagedKVCache:
         """Moves the live pages to the front and says how many they are (this waits for the device)."""
         self._owned("compact")
         self._moves[0] += 1
-        self.page_table, self.refcounts, live = ops.paged_compact(self.pages, self.page_table, self.refcounts)
+        table, self.refcounts, live = ops.paged_compact(self.pages, self.page_table, self.refcounts)
+        self._same_room(table)
         return int(live)
 
     def resize(self, num_pages: int) -> None:

@@ -545,7 +545,7 @@ def _check_paged(layers, cache: PagedKVCache, S: int, Sk: int) -> None:
         if held is None or m is None:
             continue
         dtype, heads, width = held.pages.dtype, held.pages.shape[3], held.pages.shape[5]
-        if dtype != torch.bfloat16 or heads != m.num_heads or width != m.q_proj.out_features // m.num_heads or held.n_layer != len(layers):
+        if dtype != torch.bfloat16 or heads != m.num_heads or width != m.q_proj.out_features // m.num_heads or held.n_layer < len(layers):
             raise ops.MmamdError(f"{what} holds {held.n_layer} layers of {heads} x {width} in {dtype}, the decoder has {len(layers)} of {m.num_heads} x "
                                  f"{m.q_proj.out_features // m.num_heads}, served in bfloat16")
     if S > 288 and att.q_proj.out_features // att.num_heads != 64:

@@ -146,6 +146,8 @@ def test_steps_without_a_reserve_are_stored(on_cpu, monkeypatch):
         if t == 30:
             c.fork(torch.tensor([1, 0], dtype=torch.int32), reserve=0)
             rows = rows[[1, 0]]
+        if t == 31:
+            c.resize(c.compact() + 4)
     assert c.lengths.tolist() == [40, 40] and int(c.lost) == 0
 
 
@@ -270,3 +272,26 @@ def test_views_of_pages_that_were_moved_are_refused(on_cpu):
     states.resize(19)
     with pytest.raises(ops.MmamdError, match="moved or freed"):
         holder.cross.attend(0, torch.randn(3, 1, 64))
+
+
+def test_tables_put_in_place_by_hand_are_left_alone(on_cpu, monkeypatch):
+    """A table whose pages the caller reserved with the operators: a step neither exchanges it nor asks for pages, and counts a token that has no place."""
+    dec, g = _Decoder(monkeypatch), torch.Generator().manual_seed(5)
+    c = cache(12, 48)
+    s = ops.paged_fork(c.pages, c.page_table, c.lengths, c.refcounts, torch.full((2,), -1, dtype=torch.int32), reserve=32)
+    c.page_table, c.lengths, c.refcounts = s[:3]
+    table, x = c.page_table, torch.randn(2, 40, 64, generator=g)
+    for t in range(33):
+        assert int(c.lost) == 0
+        out = dec(x[:, t:t + 1], c)
+        assert t == 32 or close(out, x[:, :t + 1])
+    assert c.page_table is table and int(c.lost) == 2
+    c.fork(torch.tensor([1], dtype=torch.int32), reserve=1)
+    held = [torch.empty_like(t) for t in (c.page_table, c.lengths, c.refcounts, c.lost)]
+    want = [t.clone() for t in (c.page_table, c.lengths, c.refcounts, c.lost)]
+    c._held_in(held)
+    assert c.page_table is held[0] and all(torch.equal(a, b) for a, b in zip(held, want))
+    dec(x[1:, 33:34], c)
+    assert c.page_table is held[0]  # the room of the fork is known in the tensors that hold its state
+    dec(x[1:, 34:35], c)
+    assert c.page_table is not held[0]
