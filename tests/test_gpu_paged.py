@@ -406,9 +406,9 @@ def test_together():
     np.testing.assert_array_equal(np.bincount(used[used >= 0].ravel(), minlength=pages), host(state.refcounts))
 
 
+@pytest.mark.parametrize("grad", [False, True], ids=["no_grad", "grad"])
 @pytest.mark.parametrize("backend", ["eager", "aot_eager"])
-@torch.no_grad()
-def test_traced_by_torch_compile(backend):
+def test_traced_by_torch_compile(backend, grad):
     """A decoding step in one graph: the operators store through views of one pool, which a graph without in-place operations (aot_eager) has to keep in order."""
     from multimodal_amd import _torch_ops
 
@@ -435,9 +435,31 @@ def test_traced_by_torch_compile(backend):
     want, pool = step(*args), args[0]
     torch._dynamo.reset()
     compiled = torch.compile(step, backend=backend, fullgraph=True)
-    for _ in range(2):
-        args = state()
-        for a, b in zip(compiled(*args), want):
-            assert torch.equal(a, b)
-        assert torch.equal(args[0], pool)
+    with torch.set_grad_enabled(grad):  # (nothing here asks for a gradient)
+        for _ in range(2):
+            args = state()
+            for a, b in zip(compiled(*args), want):
+                assert torch.equal(a, b)
+            assert torch.equal(args[0], pool)
     torch._dynamo.reset()
+
+
+def test_gradients_are_refused_on_the_device():
+    """The same refusals as on meta tensors (tests/test_decoding_no_grad.py), before anything is stored."""
+    import torch.autograd.forward_ad as fwad
+
+    kp, vp, table, q, k, v = make(3, 2, 4, 2, 64, 16, [5, 20], F32)
+    before, n = (kp.clone(), vp.clone()), i32([5, 20])
+    with pytest.raises(ops.MmamdError, match="no gradient"):
+        ops.paged_attention(q, kp, vp, table, n, k.clone().requires_grad_(), v)
+    with fwad.dual_level(), pytest.raises(ops.MmamdError, match="no gradient"):
+        ops.paged_attention(fwad.make_dual(q.contiguous(), q.contiguous()), kp, vp, table, n, k, v)
+    with pytest.raises(ops.MmamdError, match="no gradient"):
+        torch.func.grad(lambda x: ops.paged_attention(x, kp, vp, table, n, k, v).sum())(q.contiguous())
+    with pytest.raises(ops.MmamdError, match="no gradient"):
+        ops.paged_append(k[:, None].clone().requires_grad_(), v[:, None], kp, vp, table, n)
+    np.testing.assert_array_equal(host(kp), host(before[0]))
+    np.testing.assert_array_equal(host(vp), host(before[1]))
+    version = kp._version
+    ops.paged_attention(q, kp, vp, table, n, k, v)
+    assert kp._version > version
